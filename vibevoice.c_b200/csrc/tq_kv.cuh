@@ -17,10 +17,11 @@
  *           by the nearest of eight 2-D code words (3 bits a pair);
  *   the codes of values 4L .. 4L+3 are bits [nb*L, nb*(L+1)) of the vector, little endian.
  *
- * The reference builds with fast-math, so its square root, its 1 / sigma (which
- * the compiler turns into a reciprocal square root of the mean square) and its
- * division by head_dim are the hardware approximations; this file names the
- * same PTX instructions (sqrt.approx.ftz, rsqrt.approx.ftz, div.approx.ftz)
+ * The reference builds with fast-math, so its square root, its 1 / sigma and its
+ * division by head_dim are the hardware approximations that the CUDA documentation
+ * names for that flag; 1.0f / sqrtf(x) is documented to become rsqrtf(x) there, so
+ * the scale is a reciprocal square root of the mean square. This file names the
+ * instructions themselves (sqrt.approx.ftz, rsqrt.approx.ftz, div.approx.ftz)
  * and performs every other operation in the reference's order, so the bytes
  * are those of the reference's kernel on the same GPU (tests/test_tq_kv.py
  * compares them with the live kernel). The code books are the format's
@@ -336,9 +337,9 @@ __device__ __forceinline__ void tq_store16(float (&v)[16], int lane, uint8_t* ds
     const float mean_sq = fmaxf(tq_div_approx(ss, 128.0f), 1e-12f);
     const float sigma = tq_sqrt_approx(mean_sq);
     /* sigma (stored) is the approximate square root of the mean square; the scale the codes are
-     * taken against is the approximate RECIPROCAL square root of that same mean -- what the
-     * reference's fast-math build makes of 1.0f / sigma -- not a reciprocal of sigma: the two
-     * differ in the last bit often enough to move a code once in some 10^4 vectors. */
+     * taken against is the approximate RECIPROCAL square root of that same mean (see the top
+     * of the file), not a reciprocal of sigma: the two differ in the last bit often enough to
+     * move a code once in some 10^4 vectors, and the stored bytes say it is this one. */
     const float inv = tq_rsqrt_approx(mean_sq);
     uint32_t bits[4];
 #pragma unroll
