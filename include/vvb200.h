@@ -323,6 +323,133 @@ vv_status_t vvb_kv_append_dev(const vvb_kv_append_t* args, void* stream);
 vv_status_t vvb_kv_rotate_dev(void* x_fp16, int n_heads, int head_dim, int rows, void* stream);
 vv_status_t vvb_kv_unrotate_dev(void* x_fp16, int n_heads, int head_dim, int rows, void* stream);
 
+/* ---- serving: many sequences over one paged cache ------------------------ *
+ * One decode or mixed step over the pool of 64-position pages: vvb_kv_plan_dev
+ * gives each sequence the pages its new tokens need and says where every row of
+ * the ragged batch goes; per layer, vvb_kv_append_slots_dev rotates and stores
+ * those rows and vvb_attn_decode_dev attends each sequence's newest token to its
+ * whole cache. Rows of a ragged batch lie one sequence after the other. All
+ * three are capturable: lengths, tables and maps are read on the device, so a
+ * replayed graph follows them. */
+
+/** What vvb_kv_plan_dev says of a sequence (status[b]). A refused sequence keeps
+ *  its length and pages; its rows get slot -1. */
+#define VVB_KV_PLAN_OK         0
+#define VVB_KV_PLAN_NO_PAGES   1   /* fewer free pages than this and the sequences before it ask for */
+#define VVB_KV_PLAN_TABLE_FULL 2   /* lens + new_tokens > 64 * table_stride */
+#define VVB_KV_PLAN_NO_ROWS    3   /* its rows end beyond max_rows */
+
+/** Block tables, slot map and positions from request lengths. For sequence b
+ *  with lens[b] cached positions, new_tokens[b] = n:
+ *    n >= 0  the sequence gets ceil((lens + n) / 64) - ceil(lens / 64) pages from
+ *            the stack of free pages, written behind the ones its row of
+ *            block_table holds, and lens_out[b] = lens[b] + n;
+ *    n < 0   its pages go back onto the stack, lens_out[b] = 0.
+ *  Pages released by a call are pushed first, in sequence order, and may be
+ *  given out by the same call; pages are then taken from the top, in sequence
+ *  order. row_start[b] is the exclusive sum of max(n, 0) (a refused sequence's
+ *  rows count too; sums stop at INT_MAX). Row r of sequence b has positions[r] =
+ *  lens[b] + r - row_start[b] and slot_map[r] = page * 64 + position % 64; both
+ *  are -1 for the rows of a refused sequence and behind the last row, up to
+ *  max_rows. Sequences are admitted in order: one is refused for pages when the
+ *  pages asked for up to and including it exceed the stack's height, so a later
+ *  sequence is never admitted in an earlier one's place unless it needs none.
+ *  lens_out may be lens and free_count_out may be free_count; no other two
+ *  arrays may overlap. Table entries beyond a sequence's pages are not touched.
+ *  The result does not depend on timing. 1 <= table_stride <= 2^25 - 1, n_pages
+ *  <= 2^25 - 1 (VV_ERR_OVERFLOW), n_seqs <= 8192 (VV_ERR_UNSUPPORTED); n_seqs == 0
+ *  writes nothing. */
+typedef struct vvb_kv_plan {
+    const int32_t* new_tokens; /* [n_seqs] */
+    const int32_t* lens;       /* [n_seqs]; below 0 counts as 0 */
+    int32_t* lens_out;         /* [n_seqs] */
+    int32_t* block_table;      /* [n_seqs, table_stride] in/out */
+    int32_t* free_pages;       /* [n_pages] stack, bottom first, in/out */
+    const int32_t* free_count; /* [1] its height */
+    int32_t* free_count_out;   /* [1] */
+    int32_t* row_start;        /* [n_seqs + 1] */
+    int32_t* slot_map;         /* [max_rows] */
+    int32_t* positions;        /* [max_rows] */
+    int32_t* status;           /* [n_seqs] or NULL */
+    int n_seqs, table_stride, n_pages, max_rows;
+} vvb_kv_plan_t;
+
+vv_status_t vvb_kv_plan_dev(const vvb_kv_plan_t* plan, void* stream);
+
+/** vvb_kv_append_dev for the rows of several sequences: row r is rotated at
+ *  position positions[r] and stored in cache row slot_map[r] (what vvb_kv_plan_dev
+ *  writes), for every cache format, bytes as vvb_kv_append_dev's. The rotated Q
+ *  goes to q_out, which may be q. A row whose slot lies outside [0, n_slots) is
+ *  left alone: no cache row, no q_out row is written. Two rows must not name the
+ *  same slot. k_ref is one reference key for all sequences (the attention's
+ *  softmax does not change with it; its log-sum-exp is then of the stored
+ *  differences). Alignment and head_dim as vvb_kv_append_dev. */
+typedef struct vvb_kv_append_slots {
+    const void* q;             /* [rows, n_q_heads, head_dim] */
+    void* q_out;               /* [rows, n_q_heads, head_dim]; q is allowed */
+    const void* k;             /* [rows, n_kv_heads, head_dim] */
+    const void* v;             /* [rows, n_kv_heads, head_dim] */
+    const void* q_bias;        /* [n_q_heads * head_dim] or NULL */
+    const void* k_bias;        /* [n_kv_heads * head_dim] or NULL */
+    const void* v_bias;        /* [n_kv_heads * head_dim] or NULL */
+    void* k_store;             /* one layer's K cache rows, [n_slots, ...] as vvb_kv_append_t */
+    void* v_store;
+    const void* k_ref;         /* FP8 / TurboQuant: FP16 [n_kv_heads * head_dim] or NULL */
+    void* k_meta;              /* TurboQuant: FP16 [n_slots, n_kv_heads], else NULL */
+    void* v_meta;
+    const int32_t* slot_map;   /* [rows] device ints */
+    const int32_t* positions;  /* [rows] device ints */
+    int rows, n_q_heads, n_kv_heads, head_dim, n_slots;
+    float theta;
+    int kv_format;
+} vvb_kv_append_slots_t;
+
+vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* args, void* stream);
+
+/** Attention of one new token per sequence over the cache, any format of
+ *  vvb_kv_append_dev: with n = lens[b] + len_add keys of sequence b (its newest
+ *  token's among them), query head h reading cache head h / (n_q_heads / n_kv_heads),
+ *    s_j = scale * q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),
+ *    lse = m + ln sum_j e^(s_j - m),  m = max_j s_j,
+ *  every sum, the maximum and the scores in FP32. A sequence without keys (or a
+ *  head all of whose scores are -inf) gets zeros and lse = -inf. Key j lies in cache row block_table[b][j / 64] * 64 + j % 64, or with
+ *  block_table == NULL in row b * table_stride + j (table_stride: rows of the
+ *  cache per sequence). n is cut to the 64 * table_stride (table_stride) positions
+ *  that there are, and to 0 below it; keys whose row lies outside [0, n_slots)
+ *  are left out as if masked. Whatever the rows beyond n hold, NaN included, has no effect. A
+ *  single sequence of the contiguous cache takes lens = its device position
+ *  (vvb_kv_append_dev's d_position) and len_add = 1.
+ *  TurboQuant caches hold rotated vectors: q is what vvb_kv_rotate_dev made of it and out is
+ *  what vvb_kv_unrotate_dev takes, as in the reference (src/inference/decoder.c:878-901).
+ *  A reference key (k_ref) shifts all scores of a head alike and is not needed.
+ *  head_dim 64, 128 or 256 (TurboQuant: 128); n_q_heads a multiple of n_kv_heads;
+ *  q, out, the stores and scratch 16-byte aligned, k_meta and v_meta 4-byte
+ *  aligned (VV_ERR_UNSUPPORTED otherwise); n_seqs <= 8192. out may be q. scratch:
+ *  vvb_attn_decode_scratch_bytes(...) bytes of device memory whose contents need
+ *  no initialisation; calls that overlap on a GPU need one each (two captured
+ *  graphs may share one when they do not run at the same time). The work is
+ *  split over the SMs by the lengths read on the device and joined in an order
+ *  that the lengths alone decide: the same inputs give the same bits. */
+typedef struct vvb_attn_decode {
+    const void* q;             /* FP16 [n_seqs, n_q_heads, head_dim] */
+    void* out;                 /* FP16 [n_seqs, n_q_heads, head_dim] */
+    float* lse;                /* FP32 [n_seqs, n_q_heads] or NULL */
+    const void* k_store;       /* [n_slots, ...] as vvb_kv_append_t */
+    const void* v_store;
+    const void* k_meta;        /* TurboQuant: FP16 [n_slots, n_kv_heads], else NULL */
+    const void* v_meta;
+    const int32_t* block_table;/* [n_seqs, table_stride] device ints or NULL */
+    const int32_t* lens;       /* [n_seqs] device ints */
+    void* scratch;
+    size_t scratch_bytes;
+    int n_seqs, n_q_heads, n_kv_heads, head_dim, n_slots, table_stride, len_add;
+    int kv_format;
+    float scale;               /* usually 1 / sqrt(head_dim) */
+} vvb_attn_decode_t;
+
+size_t vvb_attn_decode_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim);
+vv_status_t vvb_attn_decode_dev(const vvb_attn_decode_t* args, void* stream);
+
 /** Final RMSNorm + LM head + greedy argmax in two launches (the reference
  *  issues four: vv_rmsnorm_dev, vv_lm_head_gemv_dev and vv_argmax_dev's two,
  *  src/inference/pipeline.c:1962-1978). x[K] is the last hidden row when

@@ -41,9 +41,15 @@
  * warp. Per 7B token the cache write shrinks from 4096 bytes to 528 (4-bit) ..
  * 208 (1.5-bit).
  *
- * Paged caches (template PAGED): logical position t = cache_offset + r lands in
- * row page_table[t / 64] * 64 + t % 64 of the pool (cache_row below), for every
- * format; the contiguous instantiations carry no trace of the mapping.
+ * Where a row goes (template ADDR): kAddrFlat, cache row cache_offset + r;
+ * kAddrPaged, logical position t = cache_offset + r lands in row
+ * page_table[t / 64] * 64 + t % 64 of the pool (cache_row below); kAddrSlots, a
+ * ragged batch of several sequences: row r goes to cache row slot_map[r] at RoPE
+ * position positions[r], and a row whose slot lies outside the cache (-1: the
+ * padding of a batch of fixed capacity, a refused sequence) is left alone
+ * altogether, Q included. For every format; an instantiation carries no trace of
+ * the other mappings. The slot of a row is loaded beside its data and tested at
+ * the store, so that it does not stand before the loads.
  */
 #include "fp8_kv.cuh"
 #include "rope.cuh"
@@ -75,7 +81,11 @@ struct RopeAppendArgs {
     const vec16* k_ref;       /* FP8 / TurboQuant: [n_kv_heads * head_dim] FP16 subtracted from K; may be null */
     __half* k_meta;           /* TurboQuant: [max_len, n_kv_heads] FP16 RMS of each stored K vector */
     __half* v_meta;
-    const int* page_table;    /* may be null: logical position t lives in cache row t */
+    const int* page_table;    /* kAddrPaged: page of logical position 64 i .. 64 i + 63 */
+    const int* slot_map;      /* kAddrSlots: [rows] cache row of each row, outside [0, n_slots): none */
+    const int* positions;     /* kAddrSlots: [rows] RoPE position */
+    vec16* q_out;             /* where the rotated Q goes: q itself, or (kAddrSlots) an array of its own */
+    int n_slots;
     int cache_offset;         /* cache row of row 0 (when r.d_position is null) */
     int keep_k;               /* also write the rotated K back in place */
     int v_ctas;               /* the grid's first v_ctas CTAs carry V, the rest are RoPE tiles ... */
@@ -92,11 +102,24 @@ __device__ __forceinline__ size_t cache_row(const int* page_table, int t) {
     return ((size_t)__ldg(page_table + (t >> kKvPageShift)) << kKvPageShift) + (size_t)(t & ((1 << kKvPageShift) - 1));
 }
 
+enum { kAddrFlat = 0, kAddrPaged = 1, kAddrSlots = 2 };
+
+/* Cache row of row r, -1 for none; `first` is the logical position of row 0. */
+template <int ADDR>
+__device__ __forceinline__ long long dest_row(const RopeAppendArgs& A, int first, int r) {
+    if constexpr (ADDR == kAddrSlots) {
+        const int s = __ldg(A.slot_map + r);
+        return (unsigned)s < (unsigned)A.n_slots ? (long long)s : -1ll;
+    } else {
+        return (long long)cache_row(ADDR == kAddrPaged ? A.page_table : nullptr, first + r);
+    }
+}
+
 __device__ __forceinline__ vec16 add_bias_vec(const vec16& x, const vec16& b) {
     return hadd8(x, b);      /* == widen, add, round to FP16 (vvb_device.cuh) */
 }
 
-template <int FMT, bool PAGED>
+template <int FMT, int ADDR>
 __global__ void __launch_bounds__(kRopeThreads, FMT == KV_RAW ? VVB_ROPE_APPEND_RAW_CTAS : 3)
 rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
     __shared__ __align__(16) float cos_s[kRopeTableEntries];
@@ -152,7 +175,12 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
                 for (int j = 0; j < kU; j++) {
                     if (base + j * 4 * kWarps >= nvecs) break;                    /* warp-uniform */
                     const int idx = base + j * 4 * kWarps + (lane >> 3);
-                    const bool live = idx < nvecs;
+                    bool live = idx < nvecs;
+                    long long row = 0;
+                    if (live) {
+                        row = dest_row<ADDR>(A, cache_first_v, row0v + rl);
+                        if (ADDR == kAddrSlots && row < 0) { live = false; row = 0; }
+                    }
                     if (A.v_bias && live) {
                         x[j][0] = add_bias_vec(x[j][0], __ldg(A.v_bias + h * 16 + 2 * sub));
                         x[j][1] = add_bias_vec(x[j][1], __ldg(A.v_bias + h * 16 + 2 * sub + 1));
@@ -165,7 +193,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
                         v16[2 * i] = f.x;
                         v16[2 * i + 1] = f.y;
                     }
-                    const size_t at = live ? cache_row(PAGED ? A.page_table : nullptr, cache_first_v + row0v + rl) * a.n_kv + h : 0;
+                    const size_t at = live ? (size_t)row * a.n_kv + h : 0;
                     tq_store16<FMT>(v16, lane, reinterpret_cast<uint8_t*>(A.v_cache) + at * BPV, A.v_meta + at, live, tq_cells);
                     h += step_h;
                     rl += step_r;
@@ -188,8 +216,10 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
                 if (it >= items) continue;
                 const int rl = it / cols_v;
                 const int cv = it - rl * cols_v;
+                const long long row = dest_row<ADDR>(A, cache_first_v, row0v + rl);
+                if (ADDR == kAddrSlots && row < 0) continue;
                 if (A.v_bias) x[j] = add_bias_vec(x[j], __ldg(A.v_bias + cv));
-                const size_t at = cache_row(PAGED ? A.page_table : nullptr, cache_first_v + row0v + rl) * cols_v + cv;
+                const size_t at = (size_t)row * cols_v + cv;
                 if constexpr (FMT == KV_RAW) st_stream(A.v_cache + at, x[j]);
                 else if constexpr (!kv_is_tq(FMT))
                     __stcs(reinterpret_cast<uint2*>(A.v_cache) + at, fp8_encode8<FMT>(x[j], nullptr));
@@ -239,7 +269,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
         const size_t off = (size_t)head * vph + vec;
         stride = (size_t)a.n_q * vph;
         src = a.q + off;
-        dst = a.q + off;
+        dst = A.q_out + off;
         if (A.q_bias) bias = A.q_bias + off;
     } else {
         const size_t off = (size_t)(head - a.n_q) * vph + vec;
@@ -259,6 +289,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
     /* Phase A: loads in flight. */
     vec16 lo[kRopeMaxRowsPerThread], hi[kRopeMaxRowsPerThread];
     bool live[kRopeMaxRowsPerThread];
+    int slot_of[kRopeMaxRowsPerThread];                    /* kAddrSlots */
     vec16 blo = make_uint4(0, 0, 0, 0), bhi = make_uint4(0, 0, 0, 0);
     if (col_ok && bias != nullptr) {
         blo = __ldg(bias);
@@ -272,6 +303,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             const vec16* p = src + (size_t)(row0 + rl) * stride;
             lo[m] = ld_stream(p);
             hi[m] = ld_stream(p + a.hvn);
+            if constexpr (ADDR == kAddrSlots) slot_of[m] = (int)dest_row<ADDR>(A, 0, row0 + rl);
         }
     }
 
@@ -280,7 +312,8 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
     for (int e = t; e < nrows * a.half; e += kRopeThreads) {
         const int rl = e / a.half;
         const int i = e - rl * a.half;
-        const float ang = __fmul_rn((float)(pos0 + rl), a.inv_freq[i]);
+        const int pos = (ADDR == kAddrSlots) ? __ldg(A.positions + row0 + rl) : pos0 + rl;
+        const float ang = __fmul_rn((float)pos, a.inv_freq[i]);
         sincos_f64(ang, &sin_s[e], &cos_s[e]);
     }
     __syncthreads();
@@ -289,6 +322,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
 #pragma unroll
     for (int m = 0; m < kRopeMaxRowsPerThread; m++) {
         if (!live[m]) continue;
+        if (ADDR == kAddrSlots && slot_of[m] < 0) continue;
         const int rl = slot + m * a.row_slots;
         vec16 xlo = lo[m], xhi = hi[m];
         if (bias != nullptr) {
@@ -320,15 +354,16 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             if constexpr (FMT != KV_RAW && !kv_is_tq(FMT)) {
                 /* one byte per element: vector i of the row is 8 bytes at uint2 index i */
                 uint2* d8 = reinterpret_cast<uint2*>(A.k_cache) +
-                            (cache_row(PAGED ? A.page_table : nullptr, dst_row_first + row0 + rl) * stride + (size_t)(dst - A.k_cache));
+                            ((size_t)(ADDR == kAddrSlots ? slot_of[m] : dest_row<ADDR>(A, dst_row_first, row0 + rl)) * stride +
+                             (size_t)(dst - A.k_cache));
                 const bool sub = A.k_ref != nullptr;
                 __stcs(d8, fp8_encode8<FMT>(xlo, sub ? &rlo : nullptr));
                 __stcs(d8 + a.hvn, fp8_encode8<FMT>(xhi, sub ? &rhi : nullptr));
             }
             /* (a TurboQuant launch always stages: the launcher plans the tile to fit) */
         } else {
-            const size_t drow = to_cache ? cache_row(PAGED ? A.page_table : nullptr, dst_row_first + row0 + rl)
-                                         : (size_t)(row0 + rl);
+            const size_t drow = !to_cache ? (size_t)(row0 + rl)
+                                : (size_t)(ADDR == kAddrSlots ? slot_of[m] : dest_row<ADDR>(A, dst_row_first, row0 + rl));
             vec16* d = dst + drow * stride;
             st_stream(d, xlo);
             st_stream(d + a.hvn, xhi);
@@ -363,8 +398,10 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             const int idx0 = 4 * warp + (lane >> 3);
             int rl = idx0 / heads, hk = idx0 - rl * heads;
             for (int base = 4 * warp; base < total; base += 4 * kWarps) {          /* warp-uniform */
-                const bool live = base + (lane >> 3) < total;
+                bool live = base + (lane >> 3) < total;
                 const int rs = live ? rl : 0, hs = live ? hk : 0;
+                long long row = dest_row<ADDR>(A, cache_first, row0 + rs);
+                if (ADDR == kAddrSlots && row < 0) { live = false; row = 0; }
                 const vec16* src16 = &k_stage[(rs * 2 + half_sel) * kcols + hs * a.hvn + vsel];
                 const vec16 x0 = src16[0], x1 = src16[1];
                 const int h = head0 + hs;
@@ -389,7 +426,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
                         v16[8 + 2 * i] = __fsub_rn(v16[8 + 2 * i], f1.x); v16[8 + 2 * i + 1] = __fsub_rn(v16[8 + 2 * i + 1], f1.y);
                     }
                 }
-                const size_t at = cache_row(PAGED ? A.page_table : nullptr, cache_first + row0 + rs) * a.n_kv + h;
+                const size_t at = (size_t)row * a.n_kv + h;
                 tq_store16<FMT>(v16, lane, reinterpret_cast<uint8_t*>(A.k_cache) + at * BPV, A.k_meta + at, live, tq_cells);
                 hk += step_h;
                 rl += step_r;
@@ -406,8 +443,9 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             const int ck = first_k_col + kc;
             const int hd = ck / a.hvn;
             const size_t off = (size_t)(hd - a.n_q) * vph + (size_t)(ck - hd * a.hvn) + ((rh & 1) ? (size_t)a.hvn : 0);
-            uint2* d8 = reinterpret_cast<uint2*>(A.k_cache) +
-                        (cache_row(PAGED ? A.page_table : nullptr, cache_first + row0 + rl) * stride_k + off);
+            const long long row = dest_row<ADDR>(A, cache_first, row0 + rl);
+            if (ADDR == kAddrSlots && row < 0) continue;
+            uint2* d8 = reinterpret_cast<uint2*>(A.k_cache) + ((size_t)row * stride_k + off);
             const vec16 x = k_stage[idx];
             if (A.k_ref != nullptr) {
                 const vec16 r = __ldg(A.k_ref + off);
@@ -433,7 +471,9 @@ extern "C" int vvbk_rope_append(void* q, void* k, const void* v,
                                 int rows, int n_q_heads, int n_kv_heads, int head_dim,
                                 int position_offset, int cache_offset, const int* d_position,
                                 const float* inv_freq, int keep_k, int kv_format, const void* k_ref,
-                                const int* page_table, void* k_meta, void* v_meta, void* stream) {
+                                const int* page_table, void* k_meta, void* v_meta, void* q_out,
+                                const int* slot_map, const int* positions, int n_slots, void* stream) {
+    if (!aligned16(q_out)) return (int)cudaErrorNotSupported;
     if (kv_format < KV_RAW || kv_format > KV_TQ1_5 || !aligned16(k_ref)) return (int)cudaErrorNotSupported;
     const bool tq = kv_is_tq(kv_format);
     if (tq && (head_dim != 128 || k_meta == nullptr || v_meta == nullptr || n_kv_heads > 32 ||
@@ -471,26 +511,30 @@ extern "C" int vvbk_rope_append(void* q, void* k, const void* v,
     A.k_meta = (__half*)k_meta;
     A.v_meta = (__half*)v_meta;
     A.page_table = page_table;
+    A.slot_map = slot_map;
+    A.positions = positions;
+    A.n_slots = n_slots;
+    A.q_out = q_out != nullptr ? (vec16*)q_out : (vec16*)q;
     A.cache_offset = cache_offset;
     A.keep_k = keep_k;
     const dim3 grid((unsigned)total), block(kRopeThreads);
     cudaStream_t s = (cudaStream_t)stream;
-    /* the paged mapping is a template parameter so that the contiguous cache pays nothing for it */
-#define VVB_APPEND_CASE(F)                                                                          \
-    case F:                                                                                         \
-        if (page_table == nullptr) launch_pdl(rope_append_kernel<F, false>, grid, block, 0, s, A);  \
-        else launch_pdl(rope_append_kernel<F, true>, grid, block, 0, s, A);                         \
+    /* the mapping is a template parameter so that the contiguous cache pays nothing for it */
+#define VVB_APPEND_CASE(F)                                                                               \
+    case F:                                                                                              \
+        if (slot_map != nullptr) launch_pdl(rope_append_kernel<F, kAddrSlots>, grid, block, 0, s, A);    \
+        else if (page_table == nullptr) launch_pdl(rope_append_kernel<F, kAddrFlat>, grid, block, 0, s, A); \
+        else launch_pdl(rope_append_kernel<F, kAddrPaged>, grid, block, 0, s, A);                        \
         break;
     switch (kv_format) {
+        VVB_APPEND_CASE(KV_RAW)
         VVB_APPEND_CASE(KV_E4M3)
         VVB_APPEND_CASE(KV_E5M2)
         VVB_APPEND_CASE(KV_TQ4)
         VVB_APPEND_CASE(KV_TQ3)
         VVB_APPEND_CASE(KV_TQ2)
         VVB_APPEND_CASE(KV_TQ1_5)
-        default:
-            if (page_table == nullptr) launch_pdl(rope_append_kernel<KV_RAW, false>, grid, block, 0, s, A);
-            else launch_pdl(rope_append_kernel<KV_RAW, true>, grid, block, 0, s, A);
+        default: return (int)cudaErrorNotSupported;
     }
 #undef VVB_APPEND_CASE
     g_launches.fetch_add(1, std::memory_order_relaxed);

@@ -41,14 +41,33 @@ int vvbk_rope(void* q, void* k, int rows, int n_q_heads, int n_kv_heads, int hea
  * page_table (may be null): device ints, one per 64-position page of the
  * logical sequence, giving the page's index in the cache arrays. kv_format
  * 3..6: the TurboQuant formats (head_dim 128 only); k_meta / v_meta then receive
- * one FP16 RMS per stored vector, [max_len, n_kv_heads]. */
+ * one FP16 RMS per stored vector, [max_len, n_kv_heads]. q_out (NULL: q) receives
+ * the rotated Q. slot_map != NULL: row r goes to cache row slot_map[r] (none when
+ * outside [0, n_slots)) at RoPE position positions[r]; page_table, d_position and
+ * the two offsets are then unused. */
 int vvbk_rope_append(void* q, void* k, const void* v,
                      const void* q_bias, const void* k_bias, const void* v_bias,
                      void* k_cache, void* v_cache,
                      int rows, int n_q_heads, int n_kv_heads, int head_dim,
                      int position_offset, int cache_offset, const int* d_position,
                      const float* inv_freq, int keep_k, int kv_format, const void* k_ref,
-                     const int* page_table, void* k_meta, void* v_meta, void* stream);
+                     const int* page_table, void* k_meta, void* v_meta, void* q_out,
+                     const int* slot_map, const int* positions, int n_slots, void* stream);
+
+/* The serving step's page bookkeeping (csrc/kv_plan.cu). n_seqs 1..8192,
+ * table_stride and n_pages at most 2^25 - 1. */
+int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_out, int* block_table, int* free_pages,
+                 const int* free_count, int* free_count_out, int* row_start, int* slot_map, int* positions,
+                 int* status, int n_seqs, int table_stride, int n_pages, int max_rows, void* stream);
+
+/* Attention of one new token per sequence over the cache (csrc/attn_decode.cu).
+ * Returns cudaErrorNotSupported (801) without launching for a head_dim that has
+ * no kernel. */
+size_t vvbk_attn_decode_scratch(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim);
+int vvbk_attn_decode(const void* q, void* out, float* lse, const void* k_store, const void* v_store,
+                     const void* k_meta, const void* v_meta, const int* block_table, const int* lens,
+                     void* scratch, int n_seqs, int n_q_heads, int n_kv_heads, int head_dim, int n_slots,
+                     int table_stride, int len_add, int kv_format, float scale, void* stream);
 
 /* The TurboQuant caches' rotation of Q / un-rotation of the attention output
  * (csrc/kv_rotate.cu): nvec head vectors of 128 halves, in place. */

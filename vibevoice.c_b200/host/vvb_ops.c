@@ -102,8 +102,91 @@ vv_status_t vvb_kv_append_dev(const vvb_kv_append_t* a, void* stream) {
                                      a->rows, a->n_q_heads, a->n_kv_heads, a->head_dim, a->position_offset,
                                      a->cache_offset, a->d_position, inv_freq, a->keep_k, a->kv_format,
                                      a->kv_format == VVB_KV_FP16 ? NULL : a->k_ref, a->page_table,
-                                     tq ? a->k_meta : NULL, tq ? a->v_meta : NULL, stream);
+                                     tq ? a->k_meta : NULL, tq ? a->v_meta : NULL, NULL, NULL, NULL, 0, stream);
     if (err == 801) return VV_ERR_UNSUPPORTED;   /* cudaErrorNotSupported: not vectorisable */
+    return from_cuda(err);
+}
+
+/* --------------------------------------------- serving over the paged KV cache */
+
+#define VVB_MAX_PAGES ((1 << 25) - 1)     /* positions and cache rows stay below 2^31 */
+#define VVB_MAX_SEQS 8192
+
+vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* a, void* stream) {
+    if (!a) return VV_ERR_NULL_PTR;
+    if (!a->q || !a->q_out || !a->k || !a->v || !a->k_store || !a->v_store || !a->slot_map || !a->positions)
+        return VV_ERR_NULL_PTR;
+    if (a->rows < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->head_dim <= 0 || a->n_slots < 0)
+        return VV_ERR_INVALID_ARG;
+    if (a->kv_format < VVB_KV_FP16 || a->kv_format > VVB_KV_TQ1_5) return VV_ERR_UNSUPPORTED;
+    const int tq = a->kv_format >= VVB_KV_TQ4;
+    if (tq && (!a->k_meta || !a->v_meta)) return VV_ERR_NULL_PTR;
+    if (tq && a->head_dim != 128) return VV_ERR_UNSUPPORTED;
+    if (((uintptr_t)a->slot_map & 3u) || ((uintptr_t)a->positions & 3u)) return VV_ERR_INVALID_ARG;
+    if (a->rows == 0) return VV_OK;
+    if (a->head_dim / 2 > VVB_ROPE_MAX_HALF) return VV_ERR_UNSUPPORTED;
+    float inv_freq[VVB_ROPE_MAX_HALF];
+    fill_inv_freq(inv_freq, a->head_dim, a->theta);
+    /* q and k are read only; keep_k is 0, so the kernel does not write k */
+    const int err = vvbk_rope_append((void*)(uintptr_t)a->q, (void*)(uintptr_t)a->k, a->v, a->q_bias, a->k_bias,
+                                     a->v_bias, a->k_store, a->v_store, a->rows, a->n_q_heads, a->n_kv_heads,
+                                     a->head_dim, 0, 0, NULL, inv_freq, 0, a->kv_format,
+                                     a->kv_format == VVB_KV_FP16 ? NULL : a->k_ref, NULL,
+                                     tq ? a->k_meta : NULL, tq ? a->v_meta : NULL, a->q_out, a->slot_map,
+                                     a->positions, a->n_slots, stream);
+    if (err == 801) return VV_ERR_UNSUPPORTED;   /* cudaErrorNotSupported: not vectorisable */
+    return from_cuda(err);
+}
+
+vv_status_t vvb_kv_plan_dev(const vvb_kv_plan_t* p, void* stream) {
+    if (!p) return VV_ERR_NULL_PTR;
+    if (!p->new_tokens || !p->lens || !p->lens_out || !p->block_table || !p->free_pages || !p->free_count ||
+        !p->free_count_out || !p->row_start)
+        return VV_ERR_NULL_PTR;
+    if (p->n_seqs < 0 || p->table_stride < 1 || p->n_pages < 0 || p->max_rows < 0) return VV_ERR_INVALID_ARG;
+    if (p->max_rows > 0 && (!p->slot_map || !p->positions)) return VV_ERR_NULL_PTR;
+    if (p->table_stride > VVB_MAX_PAGES || p->n_pages > VVB_MAX_PAGES) return VV_ERR_OVERFLOW;
+    if (p->n_seqs > VVB_MAX_SEQS) return VV_ERR_UNSUPPORTED;
+    const void* ints[] = {p->new_tokens, p->lens, p->lens_out, p->block_table, p->free_pages, p->free_count,
+                          p->free_count_out, p->row_start, p->slot_map, p->positions, p->status};
+    for (size_t i = 0; i < sizeof ints / sizeof ints[0]; i++)
+        if ((uintptr_t)ints[i] & 3u) return VV_ERR_INVALID_ARG;
+    if (p->n_seqs == 0) return VV_OK;
+    return from_cuda(vvbk_kv_plan(p->new_tokens, p->lens, p->lens_out, p->block_table, p->free_pages, p->free_count,
+                                  p->free_count_out, p->row_start, p->slot_map, p->positions, p->status, p->n_seqs,
+                                  p->table_stride, p->n_pages, p->max_rows, stream));
+}
+
+size_t vvb_attn_decode_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim) {
+    if (n_seqs <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 || n_q_heads % n_kv_heads != 0) return 0;
+    return vvbk_attn_decode_scratch(n_seqs, n_q_heads, n_kv_heads, head_dim);
+}
+
+vv_status_t vvb_attn_decode_dev(const vvb_attn_decode_t* a, void* stream) {
+    if (!a) return VV_ERR_NULL_PTR;
+    if (!a->q || !a->out || !a->k_store || !a->v_store || !a->lens || !a->scratch) return VV_ERR_NULL_PTR;
+    if (a->n_seqs < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->head_dim <= 0 || a->n_slots < 0 ||
+        a->table_stride < 1 || a->n_q_heads % a->n_kv_heads != 0 || !isfinite(a->scale))
+        return VV_ERR_INVALID_ARG;
+    if (a->kv_format < VVB_KV_FP16 || a->kv_format > VVB_KV_TQ1_5) return VV_ERR_UNSUPPORTED;
+    const int tq = a->kv_format >= VVB_KV_TQ4;
+    if (tq && (!a->k_meta || !a->v_meta)) return VV_ERR_NULL_PTR;
+    if (a->head_dim != 128 && (tq || (a->head_dim != 64 && a->head_dim != 256))) return VV_ERR_UNSUPPORTED;
+    if (a->block_table && a->table_stride > VVB_MAX_PAGES) return VV_ERR_OVERFLOW;
+    if (a->n_seqs > VVB_MAX_SEQS) return VV_ERR_UNSUPPORTED;
+    const void* wide[] = {a->q, a->out, a->k_store, a->v_store, a->scratch};
+    for (size_t i = 0; i < sizeof wide / sizeof wide[0]; i++)
+        if ((uintptr_t)wide[i] & 15u) return VV_ERR_UNSUPPORTED;
+    if (((uintptr_t)a->lens & 3u) || ((uintptr_t)a->lse & 3u) || ((uintptr_t)a->block_table & 3u)) return VV_ERR_INVALID_ARG;
+    if (tq && (((uintptr_t)a->k_meta & 3u) || ((uintptr_t)a->v_meta & 3u))) return VV_ERR_UNSUPPORTED;
+    if (a->scratch_bytes < vvb_attn_decode_scratch_bytes(a->n_seqs, a->n_q_heads, a->n_kv_heads, a->head_dim))
+        return VV_ERR_INVALID_ARG;
+    if (a->n_seqs == 0) return VV_OK;
+    const int err = vvbk_attn_decode(a->q, a->out, a->lse, a->k_store, a->v_store, tq ? a->k_meta : NULL,
+                                     tq ? a->v_meta : NULL, a->block_table, a->lens, a->scratch, a->n_seqs,
+                                     a->n_q_heads, a->n_kv_heads, a->head_dim, a->n_slots, a->table_stride,
+                                     a->len_add, a->kv_format, a->scale, stream);
+    if (err == 801) return VV_ERR_UNSUPPORTED;
     return from_cuda(err);
 }
 

@@ -70,9 +70,42 @@ class KvAppend(C.Structure):
     ]
 
 
+class KvPlan(C.Structure):
+    """vvb_kv_plan_t (include/vvb200.h)."""
+    _fields_ = [
+        ("new_tokens", _vp), ("lens", _vp), ("lens_out", _vp), ("block_table", _vp), ("free_pages", _vp),
+        ("free_count", _vp), ("free_count_out", _vp), ("row_start", _vp), ("slot_map", _vp), ("positions", _vp),
+        ("status", _vp), ("n_seqs", _i), ("table_stride", _i), ("n_pages", _i), ("max_rows", _i),
+    ]
+
+
+class KvAppendSlots(C.Structure):
+    """vvb_kv_append_slots_t (include/vvb200.h)."""
+    _fields_ = [
+        ("q", _vp), ("q_out", _vp), ("k", _vp), ("v", _vp), ("q_bias", _vp), ("k_bias", _vp), ("v_bias", _vp),
+        ("k_store", _vp), ("v_store", _vp), ("k_ref", _vp), ("k_meta", _vp), ("v_meta", _vp), ("slot_map", _vp),
+        ("positions", _vp), ("rows", _i), ("n_q_heads", _i), ("n_kv_heads", _i), ("head_dim", _i), ("n_slots", _i),
+        ("theta", _f), ("kv_format", _i),
+    ]
+
+
+class AttnDecode(C.Structure):
+    """vvb_attn_decode_t (include/vvb200.h)."""
+    _fields_ = [
+        ("q", _vp), ("out", _vp), ("lse", _vp), ("k_store", _vp), ("v_store", _vp), ("k_meta", _vp), ("v_meta", _vp),
+        ("block_table", _vp), ("lens", _vp), ("scratch", _vp), ("scratch_bytes", _sz), ("n_seqs", _i),
+        ("n_q_heads", _i), ("n_kv_heads", _i), ("head_dim", _i), ("n_slots", _i), ("table_stride", _i),
+        ("len_add", _i), ("kv_format", _i), ("scale", _f),
+    ]
+
+
 # name -> (restype, argtypes): every symbol include/vvb200.h declares
 SIGNATURES = {
     "vvb_kv_append_dev": (_i, [C.POINTER(KvAppend), _vp]),
+    "vvb_kv_plan_dev": (_i, [C.POINTER(KvPlan), _vp]),
+    "vvb_kv_append_slots_dev": (_i, [C.POINTER(KvAppendSlots), _vp]),
+    "vvb_attn_decode_scratch_bytes": (_sz, [_i, _i, _i, _i]),
+    "vvb_attn_decode_dev": (_i, [C.POINTER(AttnDecode), _vp]),
     "vvb_kv_rotate_dev": (_i, [_vp, _i, _i, _i, _vp]),
     "vvb_kv_unrotate_dev": (_i, [_vp, _i, _i, _i, _vp]),
     "vv_embedding_dev": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
@@ -299,6 +332,58 @@ def vvb_kv_rotate_dev(x, n_heads, head_dim, rows, stream=None) -> int:
 def vvb_kv_unrotate_dev(x, n_heads, head_dim, rows, stream=None) -> int:
     """The attention output after it: the inverse of vvb_kv_rotate_dev; in place."""
     return _lib.vvb_kv_unrotate_dev(_ptr(x), n_heads, head_dim, rows, _stream(stream))
+
+
+# serving: many sequences over one paged cache
+VVB_KV_PLAN_OK, VVB_KV_PLAN_NO_PAGES, VVB_KV_PLAN_TABLE_FULL, VVB_KV_PLAN_NO_ROWS = 0, 1, 2, 3
+
+
+def make_kv_plan(new_tokens, lens, lens_out, block_table, free_pages, free_count, free_count_out, row_start, slot_map,
+                 positions, status, n_seqs, table_stride, n_pages, max_rows) -> KvPlan:
+    """Fill a vvb_kv_plan_t from device tensors (int32; status may be None). It holds addresses only: keep the
+    tensors alive while it is used. lens_out may be lens, free_count_out may be free_count."""
+    return KvPlan(_ptr(new_tokens), _ptr(lens), _ptr(lens_out), _ptr(block_table), _ptr(free_pages), _ptr(free_count),
+                  _ptr(free_count_out), _ptr(row_start), _ptr(slot_map), _ptr(positions), _ptr(status), n_seqs,
+                  table_stride, n_pages, max_rows)
+
+
+def vvb_kv_plan_dev(plan: KvPlan, stream=None) -> int:
+    """Block tables, slot map and positions of one step from request lengths, on the device."""
+    return _lib.vvb_kv_plan_dev(C.byref(plan), _stream(stream))
+
+
+def make_kv_append_slots(q, q_out, k, v, k_store, v_store, slot_map, positions, rows, n_q_heads, n_kv_heads, head_dim,
+                         n_slots, *, q_bias=None, k_bias=None, v_bias=None, k_ref=None, theta=1e6, kv_format=0,
+                         k_meta=None, v_meta=None) -> KvAppendSlots:
+    """Fill a vvb_kv_append_slots_t from device tensors; it holds addresses only."""
+    return KvAppendSlots(_ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_bias), _ptr(k_bias), _ptr(v_bias),
+                         _ptr(k_store), _ptr(v_store), _ptr(k_ref), _ptr(k_meta), _ptr(v_meta), _ptr(slot_map),
+                         _ptr(positions), rows, n_q_heads, n_kv_heads, head_dim, n_slots, theta, kv_format)
+
+
+def vvb_kv_append_slots_dev(args: KvAppendSlots, stream=None) -> int:
+    """Bias adds + RoPE + KV-cache append of a ragged batch's rows through a slot map, in one launch."""
+    return _lib.vvb_kv_append_slots_dev(C.byref(args), _stream(stream))
+
+
+def vvb_attn_decode_scratch_bytes(n_seqs, n_q_heads, n_kv_heads, head_dim) -> int:
+    return int(_lib.vvb_attn_decode_scratch_bytes(n_seqs, n_q_heads, n_kv_heads, head_dim))
+
+
+def make_attn_decode(q, out, k_store, v_store, lens, n_seqs, n_q_heads, n_kv_heads, head_dim, n_slots, *,
+                     block_table=None, table_stride, len_add=0, scale=None, kv_format=0, k_meta=None, v_meta=None,
+                     lse=None, scratch, scratch_bytes) -> AttnDecode:
+    """Fill a vvb_attn_decode_t from device tensors; it holds addresses only. scale None: 1 / sqrt(head_dim)."""
+    if scale is None:
+        scale = head_dim ** -0.5 if head_dim > 0 else 1.0
+    return AttnDecode(_ptr(q), _ptr(out), _ptr(lse), _ptr(k_store), _ptr(v_store), _ptr(k_meta), _ptr(v_meta),
+                      _ptr(block_table), _ptr(lens), _ptr(scratch), scratch_bytes, n_seqs, n_q_heads, n_kv_heads,
+                      head_dim, n_slots, table_stride, len_add, kv_format, scale)
+
+
+def vvb_attn_decode_dev(args: AttnDecode, stream=None) -> int:
+    """Attention of one new token per sequence over its paged (or contiguous) cache."""
+    return _lib.vvb_attn_decode_dev(C.byref(args), _stream(stream))
 
 
 def vvb_rope_qk_append_fp8_dev(q, k, v, q_bias, k_bias, v_bias, k_store, v_store, k_ref, rows, n_q_heads,
