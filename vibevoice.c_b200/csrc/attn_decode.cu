@@ -45,6 +45,7 @@
 #include "vvb_launch.h"
 
 #include <atomic>
+#include <type_traits>
 
 namespace vvb {
 
@@ -52,10 +53,16 @@ extern std::atomic<uint64_t> g_launches;
 
 constexpr int kAttnPageShift = 6;
 constexpr int kAttnWarps = 4;                   /* a quarter of a 64-position block each */
-constexpr int kAttnCtas = 2 * 148;              /* parts the work is cut into */
+#ifndef VVB_ATTN_WAVES
+#define VVB_ATTN_WAVES 1
+#endif
+constexpr int kAttnParts = VVB_ATTN_WAVES * 3 * 148;      /* parts the work is cut into, at most */
+constexpr int kAttnJoinCtas = 2 * 148;
+constexpr int kAttnItemCost = 1;                /* what beginning and ending an item costs, in blocks */
 constexpr int kAttnJoinThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kWeightScale = 32768.0f;        /* weights are at most 1 */
+constexpr float kWeightLog2 = 12.0f;            /* a weight of 1 is kept as 2^12 ... */
+constexpr float kWeightTop = 15.0f;             /* ... and the maximum follows the scores once one passes 2^15 */
 constexpr float kNoMax = -3e38f;
 
 struct AttnArgs {
@@ -68,9 +75,9 @@ struct AttnArgs {
     const __half* v_meta;
     const int* block_table;    /* null: contiguous */
     const int* lens;
-    int2* desc;                /* [kAttnCtas] item that ends in this CTA and began in an earlier one, that CTA; or -1 */
-    float2* part_ml;           /* [2 kAttnCtas][heads of an item] maximum, sum */
-    float4* part_o;            /* [2 kAttnCtas][tiles][32] output, in the lanes' layout */
+    int2* desc;                /* [kAttnParts] item that ends in this CTA and began in an earlier one, that CTA; or -1 */
+    float2* part_ml;           /* [2 kAttnParts][heads of an item] maximum, sum */
+    float4* part_o;            /* [2 kAttnParts][tiles][32] output, in the lanes' layout */
     int n_seqs, n_q, n_kv, n_slots, table_stride, len_add;
     int group, head_blocks;    /* query heads to a cache head, items a cache head is cut into */
     float scale2;              /* scale * log2(e) */
@@ -107,11 +114,14 @@ template <int FMT> __host__ __device__ constexpr float attn_alpha() {
 template <int FMT, int HD, int NT> struct AttnShape {
     using F = AttnFmt<FMT, HD>;
     static constexpr int K_BYTES = 2 * F::KU * F::KN, V_BYTES = 4 * F::VU * F::VN;
-    static constexpr int LANE_BYTES = K_BYTES + V_BYTES + 4 * F::META + 4;                    /* of a stage; the last word: live rows */
-    static constexpr int STAGES = FMT == KV_RAW ? (HD == 256 ? 2 : 3) : 4;
+    static constexpr int LANE_BYTES = K_BYTES + V_BYTES + 4 * F::META;                        /* of a stage */
+    static constexpr int CTAS = HD == 256 || NT == 2 ? 2 : 3;                                 /* an SM's, by registers and shared memory */
+    static constexpr int STAGES = LANE_BYTES >= 256 ? 2 : kv_is_tq(FMT) ? 3 : 4;
     static constexpr int RING = 32 * LANE_BYTES * STAGES;                                     /* a warp's */
     static constexpr int TILES = HD / 16;                                                     /* 16-dim tiles of the output */
-    static constexpr int XCHG = kAttnWarps * (kAttnWarps - 1) * (NT * TILES / kAttnWarps) * 32 * 16;
+    static constexpr int MINE = NT * TILES / kAttnWarps;                                      /* of them a warp finishes, ... */
+    static constexpr int PER_ROUND = 1, ROUNDS = MINE / PER_ROUND;                            /* ... so many in one round of the exchange */
+    static constexpr int XCHG = kAttnWarps * (kAttnWarps - 1) * PER_ROUND * 32 * 16;
     static constexpr int LUT = F::LUT * 128;
     static constexpr int SMEM = LUT + kAttnWarps * RING + XCHG;       /* in this order */
 };
@@ -123,14 +133,14 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool live) {
-    const int n = live ? BYTES : 0;                    /* 0: the destination is filled with zeros, nothing is read */
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+/* BYTES of a row into shared memory at dst + AT; `some`: only n of them are read, the rest become zeros. */
+template <int BYTES, int AT> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(dst), "l"(src), "n"(AT) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES), "n"(AT) : "memory");
 }
-__device__ __forceinline__ void cp_async_some(uint32_t dst, const void* src, int n) {         /* n of 4 bytes */
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+template <int BYTES, int AT> __device__ __forceinline__ void cp_async_some(uint32_t dst, const void* src, int n) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %3], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(AT) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0 + %4], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n), "n"(AT) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -139,6 +149,24 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2_rz(float a, float b) {       /* two halves, rounded toward zero; low half = a */
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t hmax2_bits(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+/* Two outputs, and the log-sum-exp, from a head's sums (maximum and sum are those of weights times 2^12).
+ * A sum of zero: no keys, or none with a score above -inf. */
+__device__ __forceinline__ uint32_t attn_out(float a, float b, float sum) {
+    const float r = 1.0f / sum;
+    return sum == 0.0f ? 0u : pack2(a * r, b * r);
+}
+__device__ __forceinline__ float attn_lse(float top, float sum) {
+    return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 /* Transpose of an 8 x 8 matrix of halves held as fragments. */
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -155,10 +183,13 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
     return r;
 }
-template <int UNIT> __device__ __forceinline__ void lds_unit(uint32_t a, uint32_t* w) {
-    if constexpr (UNIT == 16) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
-    else if constexpr (UNIT == 8) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
-    else w[0] = lds32(a);
+template <int UNIT, int AT> __device__ __forceinline__ void lds_unit(uint32_t a, uint32_t* w) {
+    if constexpr (UNIT == 16)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a), "n"(AT));
+    else if constexpr (UNIT == 8)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2 + %3];" : "=r"(w[0]), "=r"(w[1]) : "r"(a), "n"(AT));
+    else
+        asm volatile("ld.shared.b32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(a), "n"(AT));
 }
 
 extern __shared__ __align__(16) uint8_t attn_smem[];           /* the code table first: its address is then a constant */
@@ -286,7 +317,7 @@ template <int FMT, int HD> __device__ __forceinline__ int attn_k_byte(int n, int
 template <int FMT, int HD> __device__ __forceinline__ int attn_v_byte(int n, int g) {
     if (FMT == KV_TQ3) return ((6 * g) & ~3) + 4 * n;
     if (FMT == KV_TQ2) return 4 * g;
-    if (FMT == KV_TQ1_5) return min(((3 * g) & ~3) + 4 * n, 20);      /* the last lane's three bytes lie in one word */
+    if (FMT == KV_TQ1_5) return ((3 * g) & ~3) + (g < 7 ? 4 * n : 0);      /* the last lane's three bytes lie in one word */
     return AttnFmt<FMT, HD>::VU == 16 ? 128 * n + 16 * g : 8 * g;
 }
 /* The odd start of a lane's bits in those words. */
@@ -306,42 +337,60 @@ __device__ __forceinline__ int attn_keys(const AttnArgs& A, int b) {
     return (int)min(min(max(n, 0ll), cap), 0x7fffffc0ll);
 }
 __device__ __forceinline__ int attn_blocks(int n) { return (n + 63) >> kAttnPageShift; }
+__device__ __forceinline__ int attn_places(int n) { return n > 0 ? attn_blocks(n) + kAttnItemCost : 0; }
+/* f(0), f(1) .. f(N - 1) with the number as a type. */
+template <int N> struct AttnUnits {
+    template <typename Fn> static __device__ __forceinline__ void each(Fn&& f) {
+        AttnUnits<N - 1>::each(f);
+        f(std::integral_constant<int, N - 1>());
+    }
+};
+template <> struct AttnUnits<0> {
+    template <typename Fn> static __device__ __forceinline__ void each(Fn&&) {}
+};
 
-/* A place in the line of blocks: block blk of item h (cache head x head block) of sequence b. */
+/* A place in the line of blocks: block blk of nb of item h (cache head x head block) of sequence b. */
 struct AttnAt {
-    int b, h, blk, n, n_next;                          /* n keys here, n_next in sequence b + 1 */
-    __device__ __forceinline__ void set(const AttnArgs& A, int seq) {
+    int b, h, hk, blk, nb, n, n_next;                  /* cache head hk; n keys here, n_next in sequence b + 1 */
+    __device__ __forceinline__ void set(const AttnArgs& A, int seq, int item, int block) {
         b = seq;
+        h = item;
+        hk = h / A.head_blocks;
+        blk = block;
         n = attn_keys(A, b);
+        nb = attn_blocks(n);
         n_next = b + 1 < A.n_seqs ? attn_keys(A, b + 1) : 0;
     }
-    __device__ __forceinline__ bool last() const { return blk + 1 >= attn_blocks(n); }        /* of the item */
-    __device__ __forceinline__ void step(const AttnArgs& A, int items) {
-        if (!last()) { blk++; return; }
+    __device__ __forceinline__ bool last() const { return blk + 1 >= nb; }                    /* of the item */
+    __device__ __forceinline__ void next_item(const AttnArgs& A, int items) {
         blk = 0;
-        if (++h < items) return;
-        h = 0;
+        if (++h < items) {
+            hk = h / A.head_blocks;
+            return;
+        }
+        h = hk = 0;
         do {
             b++;
             n = n_next;
             n_next = b + 1 < A.n_seqs ? attn_keys(A, b + 1) : 0;
         } while (n == 0 && b < A.n_seqs);
+        nb = attn_blocks(n);
     }
 };
 
 template <int FMT, int HD, int NT>
-__global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
     using F = AttnFmt<FMT, HD>;
     using S = AttnShape<FMT, HD, NT>;
     constexpr bool TQ = kv_is_tq(FMT);
-    constexpr int TILES = S::TILES, MINE = NT * TILES / kAttnWarps;    /* tiles of the output, those a warp finishes */
+    constexpr int TILES = S::TILES, MINE = S::MINE;    /* tiles of the output, those a warp finishes */
     __shared__ float m_s[kAttnWarps][8 * NT], l_s[kAttnWarps][8 * NT], f_s[kAttnWarps];
     __shared__ long long scan_s[kAttnWarps + 1];
-    __shared__ int find_s[2];
+    __shared__ int find_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t smem0 = (uint32_t)__cvta_generic_to_shared(attn_smem);
     const uint32_t ring = smem0 + S::LUT + warp * S::RING;
-    const uint32_t xchg = smem0 + S::LUT + kAttnWarps * S::RING;
+    const uint32_t xchg = smem0 + S::LUT + kAttnWarps * S::RING + 16 * lane;
     const uint32_t lane4 = 4 * lane;                   /* this lane's copy of the table */
 
     if constexpr (F::LUT > 0) {
@@ -350,12 +399,13 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
     pdl_wait();
     pdl_trigger();
 
-    /* This CTA's part of the line: sum the sequences' blocks, then find where the part begins. */
+    /* This CTA's part of the line: sum the sequences' blocks, then find where the part begins. Each
+     * item counts kAttnItemCost places more than it has blocks, ahead of its first block. */
     const int items = A.n_kv * A.head_blocks;
     const int per = (A.n_seqs + 32 * kAttnWarps - 1) / (32 * kAttnWarps);
     const int s0 = min(tid * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
     long long mine = 0;
-    for (int b = s0; b < s1; b++) mine += attn_blocks(attn_keys(A, b));
+    for (int b = s0; b < s1; b++) mine += attn_places(attn_keys(A, b));
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -371,19 +421,19 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
         total += scan_s[w];
     }
     total *= items;
-    const int parts = (int)min((long long)gridDim.x, total);
+    const int parts = (int)min((long long)gridDim.x, total / (1 + kAttnItemCost));
     const int part = blockIdx.x;
     const long long u0 = part < parts ? total * part / parts : 0, u1 = part < parts ? total * (part + 1) / parts : 0;
     if (u0 < u1 && mine > 0 && u0 >= before * items && u0 < (before + mine) * items) {
         long long at = before;                         /* one thread finds itself here */
         for (int b = s0; b < s1; b++) {
-            const int nb = attn_blocks(attn_keys(A, b));
-            if (u0 < (at + nb) * items) {
-                find_s[0] = b;
+            const int np = attn_places(attn_keys(A, b));
+            if (u0 < (at + np) * items) {
+                find_s = b;
                 scan_s[kAttnWarps] = u0 - at * items;
                 break;
             }
-            at += nb;
+            at += np;
         }
     }
     /* rows without keys */
@@ -392,28 +442,31 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
         uint32_t* o = reinterpret_cast<uint32_t*>(A.out + (size_t)b * A.n_q * HD);
         for (int i = tid; i < A.n_q * HD / 2; i += 32 * kAttnWarps) o[i] = 0;
         if (A.lse != nullptr)
-            for (int i = tid; i < A.n_q; i += 32 * kAttnWarps) A.lse[(size_t)b * A.n_q + i] = __int_as_float(0xff800000);
+            for (int i = tid; i < A.n_q; i += 32 * kAttnWarps) A.lse[(size_t)b * A.n_q + i] = -INFINITY;
     }
     __syncthreads();
-    if (tid == 0 && (u0 >= u1)) A.desc[part] = make_int2(-1, 0);
-    if (u0 >= u1) return;
 
     AttnAt to, at;                                     /* what is copied next, what is computed next */
-    to.set(A, find_s[0]);
-    {
+    int places = (int)(u1 - u0), skipped = 0;          /* of the line that are left to this CTA */
+    if (places > 0) {
         const long long in = scan_s[kAttnWarps];
-        const int nb = attn_blocks(to.n);
-        to.h = (int)(in / nb);
-        to.blk = (int)(in - (long long)to.h * nb);
+        const int b = find_s, np = attn_places(attn_keys(A, b)), item = (int)(in / np);
+        const int off = (int)(in - (long long)item * np);
+        to.set(A, b, item, max(off - kAttnItemCost, 0));
+        skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
+        places -= skipped;
+    }
+    if (places <= 0) {
+        if (tid == 0) A.desc[part] = make_int2(-1, 0);
+        return;
     }
     at = to;
     bool began = at.blk == 0;                          /* this CTA holds the beginning of the item */
     /* the item that ends here and began in an earlier CTA; which one it began in follows from the cut */
     if (tid == 0) {
         int2 d = make_int2(-1, 0);
-        const int nb = attn_blocks(at.n);
-        if (!began && u1 - u0 >= nb - at.blk) {
-            const long long first = u0 - at.blk;       /* the part that holds block `first` of the line */
+        if (!began && places >= at.nb - at.blk) {
+            const long long first = u0 + skipped - at.blk;       /* place of the item's first block */
             int p = (int)(first * parts / total);
             while (total * p / parts > first) p--;
             while (total * (p + 1) / parts <= first) p++;
@@ -422,80 +475,133 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
         A.desc[part] = d;
     }
 
-    const int steps = (int)(u1 - u0);
-    auto page_row = [&](const AttnAt& x) -> long long {            /* cache row of the block's first position */
-        if (A.block_table != nullptr)
-            return (long long)__ldg(A.block_table + (size_t)x.b * A.table_stride + x.blk) << kAttnPageShift;
-        return (long long)x.b * A.table_stride + ((long long)x.blk << kAttnPageShift);
+    /* What is copied next. A lane's K rows are g, g + 8 of the warp's 16, its V rows 2t, 2t + 1, 2t + 8,
+     * 2t + 9; the pointers are those of its bytes in row 0 of the cache. */
+    const uint32_t row_bytes = (uint32_t)A.n_kv * F::VEC;
+    const uint8_t *klane, *vlane;
+    int row_to;                                        /* cache row of the block's first position, -1: none; read one step ahead */
+    auto aim_item = [&]() {
+        klane = A.k_store + (size_t)g * row_bytes + to.hk * F::VEC + attn_k_byte<FMT, HD>(0, t);
+        vlane = A.v_store + (size_t)(2 * t) * row_bytes + to.hk * F::VEC + attn_v_byte<FMT, HD>(0, g);
     };
-    long long row_to = page_row(to);                   /* read one step ahead of its use */
-    int issued = 0;
-    auto issue = [&](int stage) {
-        if (issued < steps) {
-            const long long row0 = row_to + 16 * warp;
-            const long long left = min((long long)(to.n - (to.blk << kAttnPageShift) - 16 * warp), (long long)A.n_slots - row0);
-            const int live = row_to < 0 ? 0 : (int)max(min(left, 16ll), 0ll);
-            const int hk = to.h / A.head_blocks;
+    auto aim = [&]() {
+        if (A.block_table != nullptr) {
+            const int page = __ldg(A.block_table + (size_t)to.b * A.table_stride + to.blk);
+            row_to = (unsigned)page <= (unsigned)(A.n_slots - 1) >> kAttnPageShift ? page << kAttnPageShift : -1;
+        } else {
+            const long long row = (long long)to.b * A.table_stride + ((long long)to.blk << kAttnPageShift);
+            row_to = row < A.n_slots ? (int)row : -1;
+        }
+    };
+    aim_item();
+    aim();
+    int to_places = places;                            /* places from `to` on */
+    const bool odd_end = TQ && (((size_t)A.n_slots * A.n_kv) & 1) != 0;      /* the last RMS value stands alone in its word */
+    auto issue = [&](int stage) -> int {               /* returns how many of the warp's 16 rows hold keys */
+        int live = 0;
+        if (to_places > 0) {
             const uint32_t base = ring + stage * (32 * S::LANE_BYTES);
-            const size_t vec0 = (size_t)(live > 0 ? row0 : 0) * A.n_kv + hk;
-            const uint8_t* kp = A.k_store + vec0 * F::VEC;
-            const uint8_t* vp = A.v_store + vec0 * F::VEC;
-            const size_t row_bytes = (size_t)A.n_kv * F::VEC;
+            const uint32_t kd = base + lane * F::KU, vd = base + 32 * S::K_BYTES + lane * F::VU;
+            const uint32_t md = base + 32 * (S::K_BYTES + S::V_BYTES) + lane4;
+            const int row0 = row_to + 16 * warp;
+            live = row_to < 0 ? 0 : min(min(to.n - (to.blk << kAttnPageShift) - 16 * warp, A.n_slots - row0), 16);
+            if (live == 16 && !(TQ && odd_end && row0 + 16 >= A.n_slots)) {
+                const uint8_t* kp = klane + (size_t)(uint32_t)row0 * row_bytes;
+                const uint8_t* vp = vlane + (size_t)(uint32_t)row0 * row_bytes;
+                AttnUnits<F::KN>::each([&](auto n) {
+                    constexpr int N = decltype(n)::value;
+                    const int off = attn_k_byte<FMT, HD>(N, t) - attn_k_byte<FMT, HD>(0, t);
+                    cp_async<F::KU, N * 32 * F::KU>(kd, kp + off);
+                    cp_async<F::KU, (F::KN + N) * 32 * F::KU>(kd, kp + 8 * (size_t)row_bytes + off);
+                });
+                AttnUnits<F::VN>::each([&](auto n) {
+                    constexpr int N = decltype(n)::value;
+                    const int off = attn_v_byte<FMT, HD>(N, g) - attn_v_byte<FMT, HD>(0, g);
+                    cp_async<F::VU, N * 32 * F::VU>(vd, vp + off);
+                    cp_async<F::VU, (F::VN + N) * 32 * F::VU>(vd, vp + row_bytes + off);
+                    cp_async<F::VU, (2 * F::VN + N) * 32 * F::VU>(vd, vp + 8 * (size_t)row_bytes + off);
+                    cp_async<F::VU, (3 * F::VN + N) * 32 * F::VU>(vd, vp + 9 * (size_t)row_bytes + off);
+                });
+                if constexpr (TQ) {
+                    /* the RMS values of rows g, g + 8: the 32-bit words that hold them */
+                    const size_t at = (((size_t)(uint32_t)(row0 + g) * A.n_kv + to.hk) * 2) & ~(size_t)3;
+                    const uint8_t* mk = reinterpret_cast<const uint8_t*>(A.k_meta) + at;
+                    const uint8_t* mv = reinterpret_cast<const uint8_t*>(A.v_meta) + at;
+                    cp_async<4, 0>(md, mk);
+                    cp_async<4, 128>(md, mk + 16 * (size_t)A.n_kv);
+                    cp_async<4, 256>(md, mv);
+                    cp_async<4, 384>(md, mv + 16 * (size_t)A.n_kv);
+                }
+            } else if (live > 0) {
+                /* rows behind the last key are filled with zeros, nothing of them is read */
+                const size_t first = (size_t)(uint32_t)row0 * row_bytes;
+                AttnUnits<F::KN>::each([&](auto n) {
+                    constexpr int N = decltype(n)::value;
+                    const int off = attn_k_byte<FMT, HD>(N, t) - attn_k_byte<FMT, HD>(0, t);
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int key = g + 8 * r;
-                const uint8_t* p = kp + (key < live ? key * row_bytes : 0);
-#pragma unroll
-                for (int n = 0; n < F::KN; n++)
-                    cp_async<F::KU>(base + (r * F::KN + n) * (32 * F::KU) + lane * F::KU, p + attn_k_byte<FMT, HD>(n, t), key < live);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int key = 2 * t + (r & 1) + 8 * (r >> 1);
-                const uint8_t* p = vp + (key < live ? key * row_bytes : 0);
-#pragma unroll
-                for (int n = 0; n < F::VN; n++)
-                    cp_async<F::VU>(base + 32 * S::K_BYTES + (r * F::VN + n) * (32 * F::VU) + lane * F::VU, p + attn_v_byte<FMT, HD>(n, g), key < live);
-            }
-            if constexpr (TQ) {
-                /* the RMS values of K rows g, g + 8, then of V's: the 32-bit word that holds each; the
-                 * array's last value may stand alone in its word */
-                const size_t last = (size_t)A.n_slots * A.n_kv - 1;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int key = g + 8 * (r & 1);
-                    const size_t i = vec0 + (key < live ? (size_t)key * A.n_kv : 0);
-                    const __half* m = (r < 2 ? A.k_meta : A.v_meta) + (i & ~(size_t)1);
-                    cp_async_some(base + 32 * (S::K_BYTES + S::V_BYTES) + r * 128 + lane * 4, m, key >= live ? 0 : (i & ~(size_t)1) == last ? 2 : 4);
+                    for (int r = 0; r < 2; r++) {
+                        const bool ok = g + 8 * r < live;
+                        const uint8_t* p = ok ? klane + first + 8 * r * (size_t)row_bytes + off : A.k_store;
+                        if (r == 0) cp_async_some<F::KU, N * 32 * F::KU>(kd, p, ok ? F::KU : 0);
+                        else cp_async_some<F::KU, (F::KN + N) * 32 * F::KU>(kd, p, ok ? F::KU : 0);
+                    }
+                });
+                AttnUnits<4 * F::VN>::each([&](auto n) {
+                    constexpr int N = decltype(n)::value % F::VN, R = decltype(n)::value / F::VN, KEY = (R & 1) + 8 * (R >> 1);
+                    const int off = attn_v_byte<FMT, HD>(N, g) - attn_v_byte<FMT, HD>(0, g);
+                    const bool ok = 2 * t + KEY < live;
+                    cp_async_some<F::VU, decltype(n)::value * 32 * F::VU>(vd, ok ? vlane + first + KEY * (size_t)row_bytes + off : A.v_store, ok ? F::VU : 0);
+                });
+                if constexpr (TQ) {
+                    const size_t end = (size_t)A.n_slots * A.n_kv * 2;         /* bytes of an array */
+                    AttnUnits<4>::each([&](auto n) {
+                        constexpr int R = decltype(n)::value;
+                        const bool ok = g + 8 * (R & 1) < live;
+                        const size_t at = ok ? (((size_t)(uint32_t)(row0 + g + 8 * (R & 1)) * A.n_kv + to.hk) * 2) & ~(size_t)3 : 0;
+                        const uint8_t* p = reinterpret_cast<const uint8_t*>(R < 2 ? A.k_meta : A.v_meta) + at;
+                        cp_async_some<4, R * 128>(md, p, !ok ? 0 : at + 4 > end ? 2 : 4);
+                    });
                 }
             }
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(base + 32 * (S::LANE_BYTES - 4) + 4 * lane), "r"(live) : "memory");
-            issued++;
-            if (issued < steps) {
-                to.step(A, items);
-                row_to = page_row(to);
+            live = max(live, 0);
+            to_places--;
+            if (!to.last()) {
+                to.blk++;
+                if (to_places > 0) aim();
+            } else {
+                to_places -= kAttnItemCost;
+                if (to_places > 0) {
+                    to.next_item(A, items);
+                    aim_item();
+                    aim();
+                }
             }
         }
         cp_commit();
+        return live;
     };
+    int live_q[S::STAGES];                             /* of the stages in flight, oldest first */
 #pragma unroll
-    for (int s = 0; s < S::STAGES - 1; s++) issue(s);
+    for (int s = 0; s < S::STAGES - 1; s++) live_q[s] = issue(s);
 
     uint32_t q[NT][HD / 8];
-    float o[NT][TILES][4], m[NT][2], l[NT][2], vref = 0.0f;
-    auto begin_item = [&]() {
-        const int hk = at.h / A.head_blocks, hb = at.h - hk * A.head_blocks;
-        const int h0 = hb * 8 * NT, heads = A.group - h0;          /* heads of this block: at most 8 NT */
-        const __half* src = A.q + ((size_t)at.b * A.n_q + (size_t)hk * A.group + h0) * HD;
+    auto load_q = [&](const AttnAt& x) {
+        const int h0 = (x.h - x.hk * A.head_blocks) * 8 * NT, heads = A.group - h0;      /* of this block: at most 8 NT */
+        const __half* src = A.q + ((size_t)x.b * A.n_q + (size_t)x.hk * A.group + h0) * HD;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int n = 0; n < HD / 32; n++) {
-                uint4 x = make_uint4(0, 0, 0, 0);
+                uint4 v = make_uint4(0, 0, 0, 0);
                 if (8 * nt + g < heads)
-                    x = *reinterpret_cast<const uint4*>(src + (size_t)(8 * nt + g) * HD + attn_k_dim<FMT>(n, t));
-                q[nt][4 * n] = x.x; q[nt][4 * n + 1] = x.y; q[nt][4 * n + 2] = x.z; q[nt][4 * n + 3] = x.w;
+                    v = *reinterpret_cast<const uint4*>(src + (size_t)(8 * nt + g) * HD + attn_k_dim<FMT>(n, t));
+                q[nt][4 * n] = v.x; q[nt][4 * n + 1] = v.y; q[nt][4 * n + 2] = v.z; q[nt][4 * n + 3] = v.w;
             }
+    };
+    float o[NT][TILES][4], m[NT][2], l[NT][2], vref;   /* m: the maximum less kWeightLog2 */
+    auto begin_item = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int j = 0; j < TILES; j++)
 #pragma unroll
@@ -505,70 +611,93 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
         }
         vref = TQ ? 5.9604645e-8f : 1.0f;              /* the smallest RMS there is: 2^-24 */
     };
+    load_q(at);
     begin_item();
 
     int stage = 0;
-    for (int i = 0; i < steps; i++) {
+    for (;;) {
         cp_wait<S::STAGES - 2>();
-        issue(stage == 0 ? S::STAGES - 1 : stage - 1);             /* into the slot that the previous step emptied */
+        live_q[S::STAGES - 1] = issue(stage == 0 ? S::STAGES - 1 : stage - 1);     /* into the slot that the previous step emptied */
+        const int live = live_q[0];
+#pragma unroll
+        for (int s = 0; s + 1 < S::STAGES; s++) live_q[s] = live_q[s + 1];
         const uint32_t base = ring + stage * (32 * S::LANE_BYTES);
-        const int live = (int)lds32(base + 32 * (S::LANE_BYTES - 4) + 4 * lane);
+        const uint32_t kd = base + lane * F::KU, vd = base + 32 * S::K_BYTES + lane * F::VU;
+        if (++stage == S::STAGES) stage = 0;
+        float sk[2] = {1.0f, 1.0f}, sv[2] = {1.0f, 1.0f};
+        float s[NT][4];
         if (live > 0) {                                /* uniform over the warp */
-            float sk[2] = {1.0f, 1.0f}, sv[2] = {1.0f, 1.0f};
-            float s[NT][4];
+            uint32_t klo[HD / 8], khi[HD / 8];
             {
-                uint32_t klo[HD / 8], khi[HD / 8];
-                {
-                    uint32_t raw[2][F::KN * F::KU / 4 + 1];
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-#pragma unroll
-                        for (int n = 0; n < F::KN; n++)
-                            lds_unit<F::KU>(base + (r * F::KN + n) * (32 * F::KU) + lane * F::KU, &raw[r][n * (F::KU / 4)]);
-                        if constexpr (FMT == KV_TQ1_5) {
-                            const int sh = attn_k_shift<FMT>(t);
-                            raw[r][0] = __funnelshift_r(raw[r][0], raw[r][1], sh);
-                            raw[r][1] >>= sh;
-                        }
-                    }
-                    attn_k_words<FMT, HD>(raw[0], klo, lane4);
-                    attn_k_words<FMT, HD>(raw[1], khi, lane4);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int ks = 0; ks < HD / 16; ks += 2) {
-                        mma16816(s0, klo[2 * ks], khi[2 * ks], klo[2 * ks + 1], khi[2 * ks + 1], q[nt][2 * ks], q[nt][2 * ks + 1]);
-                        mma16816(s1, klo[2 * ks + 2], khi[2 * ks + 2], klo[2 * ks + 3], khi[2 * ks + 3], q[nt][2 * ks + 2], q[nt][2 * ks + 3]);
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; c++) s[nt][c] = s0[c] + s1[c];
-                }
-            }
-            if constexpr (TQ) {
-                const uint32_t mb = base + 32 * (S::K_BYTES + S::V_BYTES) + 4 * lane;
-                /* which half of the word: the parity of the value's index */
-                const int hk = at.h / A.head_blocks;
-                const int bk = A.block_table != nullptr ? 0 : (int)(((long long)at.b * A.table_stride) & 1);      /* 64 blk + 16 warp are even */
+                uint32_t raw[2][F::KN * F::KU / 4 + 1];
+                AttnUnits<F::KN>::each([&](auto n) {
+                    constexpr int N = decltype(n)::value;
+                    lds_unit<F::KU, N * 32 * F::KU>(kd, &raw[0][N * (F::KU / 4)]);
+                    lds_unit<F::KU, (F::KN + N) * 32 * F::KU>(kd, &raw[1][N * (F::KU / 4)]);
+                });
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const int odd = ((bk + g + 8 * r) * A.n_kv + hk) & 1;
-                    const uint32_t wk = lds32(mb + 128 * r), wv = lds32(mb + 128 * (2 + r));
-                    sk[r] = __half2float(__ushort_as_half((unsigned short)(odd ? wk >> 16 : wk)));
-                    sv[r] = __half2float(__ushort_as_half((unsigned short)(odd ? wv >> 16 : wv)));
+                    if constexpr (FMT == KV_TQ1_5) {
+                        const int sh = attn_k_shift<FMT>(t);
+                        raw[r][0] = __funnelshift_r(raw[r][0], raw[r][1], sh);
+                        raw[r][1] >>= sh;
+                    }
+                }
+                attn_k_words<FMT, HD>(raw[0], klo, lane4);
+                attn_k_words<FMT, HD>(raw[1], khi, lane4);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ks += 2) {
+                    mma16816(s0, klo[2 * ks], khi[2 * ks], klo[2 * ks + 1], khi[2 * ks + 1], q[nt][2 * ks], q[nt][2 * ks + 1]);
+                    mma16816(s1, klo[2 * ks + 2], khi[2 * ks + 2], klo[2 * ks + 3], khi[2 * ks + 3], q[nt][2 * ks + 2], q[nt][2 * ks + 3]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[nt][c] = s0[c] + s1[c];
+            }
+        }
+        /* the next item's Q is on its way while this one is finished */
+        const bool item_done = at.last();
+        places--;
+        const bool more = item_done ? places > kAttnItemCost : places > 0;
+        AttnAt nx = at;
+        if (!item_done) {
+            nx.blk++;
+        } else if (more) {
+            nx.next_item(A, items);
+            load_q(nx);
+        }
+        if (live > 0) {
+            if constexpr (TQ) {
+                const uint32_t mb = base + 32 * (S::K_BYTES + S::V_BYTES) + lane4;
+                /* which half of the word: the parity of the value's index (64 blk + 16 warp + 8 are even) */
+                const int bk = A.block_table != nullptr ? 0 : (int)(((long long)at.b * A.table_stride) & 1);
+                const int shift = (((bk + g) * A.n_kv + at.hk) & 1) * 16;
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    sk[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb + 128 * r) >> shift)));
+                    sv[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb + 128 * (2 + r)) >> shift)));
                 }
             }
             /* scores in base 2; rows behind the last key have none */
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[nt][c] *= TQ ? A.scale2 * (sk[c >> 1] * (1.0f / attn_alpha<FMT>())) : A.scale2;
+            if (live < 16) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (g + 8 * (c >> 1) >= live) s[nt][c] = -INFINITY;
+            }
             bool up = false;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const float f = TQ ? A.scale2 * (sk[c >> 1] * (1.0f / attn_alpha<FMT>())) : A.scale2;
-                    s[nt][c] = g + 8 * (c >> 1) < live ? s[nt][c] * f : -INFINITY;
-                    up |= s[nt][c] > m[nt][c & 1];
-                }
+                for (int c = 0; c < 4; c++) up |= s[nt][c] > m[nt][c & 1] + kWeightTop;
             if constexpr (TQ) up |= fmaxf(sv[0], sv[1]) > vref;
             if (__any_sync(0xffffffffu, up)) {
                 /* a new maximum (or a larger RMS of V): rescale what there is */
@@ -591,7 +720,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        x = fmaxf(x, m[nt][c]);
+                        x = fmaxf(x - kWeightLog2, m[nt][c]);
                         const float a = ex2(m[nt][c] - x);
                         m[nt][c] = x;
                         l[nt][c] *= a;
@@ -604,32 +733,34 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
             }
             /* weights: FP32 sums, FP16 pairs for the product */
             uint32_t bh[NT][2], bl[NT][2];
-            const float inv = TQ ? kWeightScale / vref : kWeightScale;
+            const float inv = 1.0f / vref;             /* (a power of two) */
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    float hi[2], lo[2];
+                    float w[2];
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        const float p = ex2(s[nt][2 * r + c] - m[nt][c]);
-                        l[nt][c] += p;
-                        const float w = TQ ? p * (sv[r] * inv) : p * kWeightScale;
-                        hi[c] = __half2float(__float2half_rz(w));
-                        lo[c] = w > 0.0f ? fmaxf(w - hi[c], 5.9604645e-8f) : w - hi[c];
+                        w[c] = ex2(s[nt][2 * r + c] - m[nt][c]);
+                        l[nt][c] += w[c];
+                        if constexpr (TQ) w[c] *= sv[r] * inv;
                     }
-                    bh[nt][r] = movmatrix(pack2(hi[0], hi[1]));
-                    bl[nt][r] = movmatrix(pack2(lo[0], lo[1]));
+                    const uint32_t hi = pack2_rz(w[0], w[1]);
+                    const float2 h = unpack2(hi);
+                    const uint32_t lo = hmax2_bits(pack2(w[0] - h.x, w[1] - h.y), 0x00010001u);      /* at least 2^-24 */
+                    bh[nt][r] = movmatrix(hi);
+                    bl[nt][r] = movmatrix(lo);
                 }
             {
                 uint32_t xa[HD / 8], xc[HD / 8];       /* keys (2t, 2t+1), (2t+8, 2t+9) */
                 {
                     uint32_t raw[4][F::VN * F::VU / 4];
+                    AttnUnits<4 * F::VN>::each([&](auto n) {
+                        constexpr int N = decltype(n)::value;
+                        lds_unit<F::VU, N * 32 * F::VU>(vd, &raw[N / F::VN][N % F::VN * (F::VU / 4)]);
+                    });
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-#pragma unroll
-                        for (int n = 0; n < F::VN; n++)
-                            lds_unit<F::VU>(base + 32 * S::K_BYTES + (r * F::VN + n) * (32 * F::VU) + lane * F::VU, &raw[r][n * (F::VU / 4)]);
                         if constexpr (FMT == KV_TQ3 || FMT == KV_TQ1_5) {
                             const int sh = attn_v_shift<FMT>(g);
                             raw[r][0] = __funnelshift_r(raw[r][0], raw[r][1], sh);
@@ -648,116 +779,110 @@ __global__ void __launch_bounds__(32 * kAttnWarps, 2) attn_decode_kernel(const _
                     }
             }
         }
-        if (++stage == S::STAGES) stage = 0;
-
-        const bool item_done = at.last();
-        if (item_done || i + 1 == steps) {
-            /* join the four warps: warp d finishes tiles d * MINE .. + MINE - 1 */
+        if (!item_done && more) {
+            at = nx;
+            continue;
+        }
+        /* the item (or the part) ends: join the four warps; warp d finishes tiles d * MINE .. + MINE - 1 */
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 4);
-                    l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
-                    l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
-                }
-            __syncthreads();                           /* the previous item's exchange has been read */
+            for (int c = 0; c < 2; c++) {
+                l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 4);
+                l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
+                l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
+            }
+        const int h0 = (at.h - at.hk * A.head_blocks) * 8 * NT, heads = A.group - h0;
+        const size_t head0 = (size_t)at.b * A.n_q + (size_t)at.hk * A.group + h0;
+        const bool whole = began && item_done;
+        const int slot = 2 * part + (began ? 1 : 0);               /* an item that began here is this CTA's last */
+        float top[NT][2], sum[NT][2], f[NT][kAttnWarps][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                if (g == 0) {
+        for (int round = 0; round < S::ROUNDS; round++) {
+            __syncthreads();                           /* what the exchange held has been read */
+            if (round == 0) {
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        m_s[warp][8 * nt + 2 * t + c] = m[nt][c];
-                        l_s[warp][8 * nt + 2 * t + c] = l[nt][c];
+                for (int nt = 0; nt < NT; nt++)
+                    if (g == 0) {
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            m_s[warp][8 * nt + 2 * t + c] = m[nt][c];
+                            l_s[warp][8 * nt + 2 * t + c] = l[nt][c];
+                        }
                     }
-                }
-            if (lane == 0) f_s[warp] = vref;
+                if (lane == 0) f_s[warp] = vref;
+            }
 #pragma unroll
             for (int x = 0; x < NT * TILES; x++) {
                 const int d = x / MINE, k = (warp - d - 1) & (kAttnWarps - 1);
+                if ((x % MINE) / S::PER_ROUND != round) continue;
                 if (d != warp) {
                     const float(&v)[4] = o[x / TILES][x % TILES];
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(xchg + (((d * (kAttnWarps - 1) + k) * MINE + x % MINE) * 32 + lane) * 16),
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(xchg + ((d * (kAttnWarps - 1) + k) * S::PER_ROUND + x % S::PER_ROUND) * 512),
                                  "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
                 }
             }
             __syncthreads();
-            const int hk = at.h / A.head_blocks, hb = at.h - hk * A.head_blocks;
-            const int heads = A.group - hb * 8 * NT;
-            const size_t head0 = (size_t)at.b * A.n_q + (size_t)hk * A.group + hb * 8 * NT;
-            const bool whole = began && item_done;
-            const int slot = 2 * part + (began ? 1 : 0);           /* an item that began here is this CTA's last */
+            if (round == 0) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float top[2], sum[2], f[kAttnWarps][2];
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const int h = 8 * nt + 2 * t + c;
-                    top[c] = m_s[0][h];
-#pragma unroll
-                    for (int w = 1; w < kAttnWarps; w++) top[c] = fmaxf(top[c], m_s[w][h]);
-                    sum[c] = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < kAttnWarps; w++) {
-                        f[w][c] = ex2(m_s[w][h] - top[c]);
-                        sum[c] += f[w][c] * l_s[w][h];
-                        f[w][c] *= f_s[w] * (1.0f / (kWeightScale * attn_alpha<FMT>()));
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < NT * TILES; x++) {
-                    if (x / TILES != nt || x / MINE != warp) continue;
-                    const int j = x % TILES;
-                    float acc[4];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[c] = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < kAttnWarps; w++) {         /* in warp order, whoever adds */
-                        float v[4];
-                        if (w == warp) {
-#pragma unroll
-                            for (int c = 0; c < 4; c++) v[c] = o[nt][j][c];
-                        } else {
-                            const int k = (w - warp - 1) & (kAttnWarps - 1);
-                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                                         : "r"(xchg + (((warp * (kAttnWarps - 1) + k) * MINE + x % MINE) * 32 + lane) * 16));
-                        }
-#pragma unroll
-                        for (int c = 0; c < 4; c++) acc[c] = fmaf(v[c], f[w][c & 1], acc[c]);
-                    }
-                    if (whole) {
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const int h = 8 * nt + 2 * t + c;
-                            if (h < heads) {
-                                const float r = sum[c] == 0.0f ? 0.0f : 1.0f / sum[c];
-                                *reinterpret_cast<uint32_t*>(A.out + (head0 + h) * HD + attn_v_dim<FMT, HD>(j, g)) =
-                                    pack2(sum[c] == 0.0f ? 0.0f : acc[c] * r, sum[c] == 0.0f ? 0.0f : acc[c + 2] * r);
-                            }
-                        }
-                    } else {
-                        A.part_o[((size_t)slot * (NT * TILES) + x) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                    }
-                }
-                if (warp == 0 && g == 0) {
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const int h = 8 * nt + 2 * t + c;
-                        if (!whole) A.part_ml[(size_t)slot * (8 * NT) + h] = make_float2(top[c], sum[c]);
-                        else if (A.lse != nullptr && h < heads)
-                            A.lse[head0 + h] = sum[c] == 0.0f ? -INFINITY : (top[c] + log2f(sum[c])) * kLn2;
+                        top[nt][c] = m_s[0][h];
+#pragma unroll
+                        for (int w = 1; w < kAttnWarps; w++) top[nt][c] = fmaxf(top[nt][c], m_s[w][h]);
+                        sum[nt][c] = 0.0f;
+#pragma unroll
+                        for (int w = 0; w < kAttnWarps; w++) {
+                            f[nt][w][c] = ex2(m_s[w][h] - top[nt][c]);
+                            sum[nt][c] += f[nt][w][c] * l_s[w][h];
+                            f[nt][w][c] *= f_s[w] * (1.0f / attn_alpha<FMT>());
+                        }
+                        if (warp == 0 && g == 0) {
+                            if (!whole) A.part_ml[(size_t)slot * (8 * NT) + h] = make_float2(top[nt][c], sum[nt][c]);
+                            else if (A.lse != nullptr && h < heads) A.lse[head0 + h] = attn_lse(top[nt][c], sum[nt][c]);
+                        }
                     }
+            }
+#pragma unroll
+            for (int x = 0; x < NT * TILES; x++) {
+                if ((x % MINE) / S::PER_ROUND != round || x / MINE != warp) continue;
+                const int nt = x / TILES, j = x % TILES;
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < kAttnWarps; w++) { /* in warp order, whoever adds */
+                    float v[4];
+                    if (w == warp) {
+#pragma unroll
+                        for (int c = 0; c < 4; c++) v[c] = o[nt][j][c];
+                    } else {
+                        const int k = (w - warp - 1) & (kAttnWarps - 1);
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                                     : "r"(xchg + ((warp * (kAttnWarps - 1) + k) * S::PER_ROUND + x % S::PER_ROUND) * 512));
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) acc[c] = fmaf(v[c], f[nt][w][c & 1], acc[c]);
+                }
+                if (whole) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int h = 8 * nt + 2 * t + c;
+                        if (h < heads)
+                            *reinterpret_cast<uint32_t*>(A.out + (head0 + h) * HD + attn_v_dim<FMT, HD>(j, g)) =
+                                attn_out(acc[c], acc[c + 2], sum[nt][c]);
+                    }
+                } else {
+                    A.part_o[((size_t)slot * (NT * TILES) + x) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 }
             }
-            if (i + 1 < steps) {
-                at.step(A, items);
-                began = true;
-                begin_item();
-            }
-        } else {
-            at.step(A, items);
         }
+        if (!more) break;
+        places -= kAttnItemCost;
+        at = nx;
+        began = true;
+        begin_item();
     }
     cp_wait<0>();
 }
@@ -771,11 +896,12 @@ __global__ void __launch_bounds__(kAttnJoinThreads) attn_join_kernel(const __gri
     __shared__ float top_s[8], sum_s[8];
     __shared__ float4 acc_s[kAttnJoinThreads / 32][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int part = blockIdx.x, nt = blockIdx.y;
+    const int nt = blockIdx.y;
     pdl_wait();
     pdl_trigger();
+    for (int part = blockIdx.x; part < kAttnParts; part += gridDim.x) {
     const int2 d = A.desc[part];
-    if (d.x < 0) return;
+    if (d.x < 0) continue;
     const int first = d.y, pieces = part - first + 1;
     auto slot_of = [&](int p) { return p == 0 ? 2 * first + 1 : 2 * (first + p); };
     if (warp < 8) {                                    /* head `warp` of the item */
@@ -823,13 +949,13 @@ __global__ void __launch_bounds__(kAttnJoinThreads) attn_join_kernel(const __gri
         for (int c = 0; c < 2; c++) {
             const int h = 8 * nt + 2 * t + c;
             if (h >= heads) continue;
-            const float sum = sum_s[2 * t + c], r = sum == 0.0f ? 0.0f : 1.0f / sum;
-            *reinterpret_cast<uint32_t*>(A.out + (head0 + h) * HD + attn_v_dim<FMT, HD>(j, g)) =
-                pack2(sum == 0.0f ? 0.0f : a[c] * r, sum == 0.0f ? 0.0f : a[c + 2] * r);
+            *reinterpret_cast<uint32_t*>(A.out + (head0 + h) * HD + attn_v_dim<FMT, HD>(j, g)) = attn_out(a[c], a[c + 2], sum_s[2 * t + c]);
         }
     }
     if (A.lse != nullptr && tid < 8 && 8 * nt + tid < heads)
-        A.lse[head0 + 8 * nt + tid] = sum_s[tid] == 0.0f ? -INFINITY : (top_s[tid] + log2f(sum_s[tid])) * kLn2;
+        A.lse[head0 + 8 * nt + tid] = attn_lse(top_s[tid], sum_s[tid]);
+    __syncthreads();
+    }
 }
 
 /* Column tiles of 8 query heads an item holds: two where the group has more than eight heads
@@ -840,9 +966,9 @@ struct AttnScratch { size_t ml, o, bytes; };
 static AttnScratch attn_scratch(int group, int head_dim) {
     const size_t heads = 8 * (size_t)attn_col_tiles(group, head_dim);
     AttnScratch s;
-    s.ml = kAttnCtas * sizeof(int2);                                   /* 16-byte multiples */
-    s.o = s.ml + 2 * kAttnCtas * heads * sizeof(float2);
-    s.bytes = s.o + 2 * kAttnCtas * heads * head_dim * sizeof(float);
+    s.ml = kAttnParts * sizeof(int2);                                   /* 16-byte multiples */
+    s.o = s.ml + 2 * kAttnParts * heads * sizeof(float2);
+    s.bytes = s.o + 2 * kAttnParts * heads * head_dim * sizeof(float);
     return s;
 }
 
@@ -851,9 +977,9 @@ static cudaError_t launch_attn(const AttnArgs& A, cudaStream_t s) {
     constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM;
     cudaError_t e = cudaFuncSetAttribute((const void*)attn_decode_kernel<FMT, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(kAttnCtas), dim3(32 * kAttnWarps), (size_t)SMEM, s, A);
+    e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(kAttnParts), dim3(32 * kAttnWarps), (size_t)SMEM, s, A);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attn_join_kernel<FMT, HD, NT>, dim3(kAttnCtas, NT), dim3(kAttnJoinThreads), 0, s, A);
+    e = launch_pdl(attn_join_kernel<FMT, HD, NT>, dim3(kAttnJoinCtas, NT), dim3(kAttnJoinThreads), 0, s, A);
     if (e == cudaSuccess) g_launches.fetch_add(2, std::memory_order_relaxed);
     return e;
 }
