@@ -45,7 +45,6 @@
 #include "vvb_launch.h"
 
 #include <atomic>
-#include <type_traits>
 
 namespace vvb {
 
@@ -55,6 +54,10 @@ constexpr int kAttnPageShift = 6;
 constexpr int kAttnWarps = 4;                   /* a quarter of a 64-position block each */
 #ifndef VVB_ATTN_WAVES
 #define VVB_ATTN_WAVES 1
+#endif
+#ifndef VVB_ATTN_CTAS
+#define VVB_ATTN_CTAS(FMT, HD, NT) (HD == 256 || NT == 2 ? 2 : 3)
+#define VVB_ATTN_STAGES(FMT, HD, NT) (AttnFmt<FMT, HD>::VEC >= 256 ? 2 : kv_is_tq(FMT) ? 3 : 4)
 #endif
 constexpr int kAttnParts = VVB_ATTN_WAVES * 3 * 148;      /* parts the work is cut into, at most */
 constexpr int kAttnJoinCtas = 2 * 148;
@@ -85,25 +88,18 @@ struct AttnArgs {
 
 /* ---------------------------------------------------------------- formats */
 
-/* What a lane copies of a group of 16 keys: KN units of KU bytes of each of its two K rows,
- * VN units of VU bytes of each of its four V rows. */
+/* Rows of a group of 16 keys in shared memory: VEC bytes each, copied in units of UNIT. Where a row is 2, 4
+ * or more 16-byte pieces the fragments are read with ldmatrix and the pieces are permuted for it (attn_place);
+ * rows of 48 and 24 bytes lie as they are in the cache and are read in 32-bit words. */
 template <int FMT, int HD> struct AttnFmt {
-    static constexpr int VEC = FMT == KV_RAW ? 2 * HD : HD;      /* bytes of a stored vector */
-    static constexpr int KU = 16, KN = VEC / 64;
-    static constexpr int VU = VEC >= 128 ? 16 : 8, VN = VEC >= 128 ? VEC / 128 : 1;
-    static constexpr int META = 0, LUT = 0;
-};
-template <int HD> struct AttnFmt<KV_TQ4, HD> {
-    static constexpr int VEC = 64, KU = 16, KN = 1, VU = 8, VN = 1, META = 4, LUT = 256;      /* two codes -> two levels */
-};
-template <int HD> struct AttnFmt<KV_TQ3, HD> {
-    static constexpr int VEC = 48, KU = 4, KN = 3, VU = 4, VN = 2, META = 4, LUT = 64;
-};
-template <int HD> struct AttnFmt<KV_TQ2, HD> {
-    static constexpr int VEC = 32, KU = 8, KN = 1, VU = 4, VN = 1, META = 4, LUT = 16;
-};
-template <int HD> struct AttnFmt<KV_TQ1_5, HD> {
-    static constexpr int VEC = 24, KU = 4, KN = 2, VU = 4, VN = 2, META = 4, LUT = 8 + 128;   /* code -> pair; two keys' codes -> two pairs */
+    static constexpr int VEC = kv_is_tq(FMT) ? tq_bytes_per_vec(FMT) : FMT == KV_RAW ? 2 * HD : HD;
+    static constexpr bool MAT = FMT != KV_TQ3 && FMT != KV_TQ1_5;
+    static constexpr int UNIT = FMT == KV_TQ1_5 ? 8 : 16;
+    static constexpr int PER_ROW = VEC / UNIT, UNITS = 16 * PER_ROW, COPIES = (UNITS + 31) / 32;      /* of a group, copies a lane makes */
+    /* dims of a word that ldmatrix brings: of K a lane's 4 bytes, of V the 2 bytes of one key */
+    static constexpr int K_DIMS = FMT == KV_RAW ? 2 : FMT == KV_TQ4 ? 8 : FMT == KV_TQ2 ? 16 : 4;
+    /* entries of the code table: two codes -> two levels; 1.5 bits: code -> pair, then two keys' codes -> two pairs */
+    static constexpr int LUT = FMT == KV_TQ4 ? 256 : FMT == KV_TQ3 ? 64 : FMT == KV_TQ2 ? 16 : FMT == KV_TQ1_5 ? 8 + 128 : 0;
 };
 
 /* Factor that brings all the levels of a code book near FP16 values. */
@@ -113,11 +109,11 @@ template <int FMT> __host__ __device__ constexpr float attn_alpha() {
 
 template <int FMT, int HD, int NT> struct AttnShape {
     using F = AttnFmt<FMT, HD>;
-    static constexpr int K_BYTES = 2 * F::KU * F::KN, V_BYTES = 4 * F::VU * F::VN;
-    static constexpr int LANE_BYTES = K_BYTES + V_BYTES + 4 * F::META;                        /* of a stage */
-    static constexpr int CTAS = HD == 256 || NT == 2 ? 2 : 3;                                 /* an SM's, by registers and shared memory */
-    static constexpr int STAGES = LANE_BYTES >= 256 ? 2 : kv_is_tq(FMT) ? 3 : 4;
-    static constexpr int RING = 32 * LANE_BYTES * STAGES;                                     /* a warp's */
+    static constexpr int ROWS = 16 * F::VEC;                                                  /* bytes of a group's K, or V */
+    static constexpr int STAGE = 2 * ROWS + (kv_is_tq(FMT) ? 512 : 0);                        /* then its RMS values, a lane's own words */
+    static constexpr int CTAS = VVB_ATTN_CTAS(FMT, HD, NT);                                   /* an SM's, by registers and shared memory */
+    static constexpr int STAGES = VVB_ATTN_STAGES(FMT, HD, NT);
+    static constexpr int RING = STAGE * STAGES;                                               /* a warp's */
     static constexpr int TILES = HD / 16;                                                     /* 16-dim tiles of the output */
     static constexpr int MINE = NT * TILES / kAttnWarps;                                      /* of them a warp finishes, ... */
     static constexpr int PER_ROUND = 1, ROUNDS = MINE / PER_ROUND;                            /* ... so many in one round of the exchange */
@@ -133,14 +129,14 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-/* BYTES of a row into shared memory at dst + AT; `some`: only n of them are read, the rest become zeros. */
-template <int BYTES, int AT> __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(dst), "l"(src), "n"(AT) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES), "n"(AT) : "memory");
+/* BYTES of global memory to shared memory at dst + AT; `some`: only n of them are read, the rest become zeros. */
+template <int BYTES> __device__ __forceinline__ void cp_async(uint32_t dst, int at, const void* src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + at), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + at), "l"(src), "n"(BYTES) : "memory");
 }
-template <int BYTES, int AT> __device__ __forceinline__ void cp_async_some(uint32_t dst, const void* src, int n) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %3], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(AT) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0 + %4], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n), "n"(AT) : "memory");
+template <int BYTES> __device__ __forceinline__ void cp_async_some(uint32_t dst, int at, const void* src, int n) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + at), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst + at), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -178,21 +174,22 @@ template <int FMT> __device__ __forceinline__ uint32_t fp8_pair(uint32_t two) { 
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, FMT == KV_E4M3 ? __NV_E4M3 : __NV_E5M2);
     return (uint32_t)h.x | ((uint32_t)h.y << 16);
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+__device__ __forceinline__ uint32_t lds32(uint32_t a, int at = 0) {
     uint32_t r;
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a + at));
     return r;
 }
-template <int UNIT, int AT> __device__ __forceinline__ void lds_unit(uint32_t a, uint32_t* w) {
-    if constexpr (UNIT == 16)
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a), "n"(AT));
-    else if constexpr (UNIT == 8)
-        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2 + %3];" : "=r"(w[0]), "=r"(w[1]) : "r"(a), "n"(AT));
-    else
-        asm volatile("ld.shared.b32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(a), "n"(AT));
+/* Four 8 x 8 matrices of 16-bit values; lane l gives the address of row l % 8 of matrix l / 8. */
+__device__ __forceinline__ void ldmatrix4(uint32_t a, int at, uint32_t (&w)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a + at));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t a, int at, uint32_t (&w)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a + at));
 }
 
-extern __shared__ __align__(16) uint8_t attn_smem[];           /* the code table first: its address is then a constant */
+extern __shared__ __align__(128) uint8_t attn_smem[];           /* the code table first: its address is then a constant */
 /* Entry c / 128 of the code table, this lane's copy (c a multiple of 128 below the table's size). */
 __device__ __forceinline__ uint32_t attn_lut(uint32_t c, uint32_t mask, uint32_t lane4, int from = 0) {
     return *reinterpret_cast<const uint32_t*>(attn_smem + from + ((c & mask) | lane4));
@@ -222,110 +219,181 @@ template <int FMT> __device__ __forceinline__ uint32_t attn_lut_entry(int e) {
 
 /* ---------------------------------------------------------------- fragments */
 
-/* First dim of the 8 that words 4n .. 4n+3 of a lane's K row (as halves) hold. */
-template <int FMT> __device__ __forceinline__ int attn_k_dim(int n, int t) {
-    return FMT == KV_RAW ? 32 * n + 8 * t : kv_is_tq(FMT) ? 32 * t + 8 * n : 64 * (n >> 1) + 16 * t + 8 * (n & 1);
+/* Place of 16-byte piece c of row `row`: the eight rows an ldmatrix reads at one c lie in eight different
+ * 16-byte banks. The permutation is an exclusive or of the piece's low bits with bits of the row. */
+template <int VEC> __host__ __device__ constexpr int attn_place(int row, int c) {
+    return VEC >= 128 ? row * VEC + ((c ^ (row & 7)) << 4)
+         : VEC == 64 ? row * 64 + ((c ^ ((row >> 1) & 3)) << 4)
+                     : row * VEC + ((c ^ ((row >> 2) & 1)) << 4);
 }
-/* Dim of value 2 j (2 j + 1 follows) of a lane's V row. */
-template <int FMT, int HD> __device__ __forceinline__ int attn_v_dim(int j, int g) {
-    if (FMT == KV_RAW) return 64 * (j >> 2) + 8 * g + 2 * (j & 3);
-    if (HD == 64) return 8 * g + 2 * j;
-    return 128 * (j >> 3) + 16 * g + 2 * (j & 7);
+/* The same for piece 2p + c, given a lane's address for piece c (the shared memory is 128-byte aligned). */
+template <int VEC> __device__ __forceinline__ uint32_t attn_pair(uint32_t a, int p) { return a ^ (32u * (p & (VEC >= 128 ? 3 : 1))); }
+__host__ __device__ constexpr int attn_pair_at(int p) { return 128 * (p >> 2); }
+
+/* Dim of half 0 of word i of a lane's K row (half 1 is the next dim). */
+template <int FMT> __device__ __forceinline__ int attn_k_dim(int i, int t) {
+    constexpr int D = AttnFmt<FMT, 128>::K_DIMS;
+    return AttnFmt<FMT, 128>::MAT ? (i / (D / 2)) * 4 * D + t * D + 2 * (i % (D / 2)) : 32 * t + 2 * i;
+}
+/* Dim of value e of a lane's V rows. */
+template <int FMT> __device__ __forceinline__ int attn_v_dim(int e, int g) {
+    constexpr int D = AttnFmt<FMT, 128>::K_DIMS / 2;
+    return AttnFmt<FMT, 128>::MAT ? (e / D) * 8 * D + g * D + e % D : 16 * g + e;
 }
 
-/* A lane's K row as halves: word i holds dims attn_k_dim(i / 4) + 2 (i % 4), + 1. */
+/* Two dims' codes at bit `bit` of words w -> two halves. */
+template <int FMT> __device__ __forceinline__ uint32_t attn_decode2(const uint32_t* w, int bit, uint32_t lane4) {
+    constexpr int NB = FMT == KV_TQ4 ? 8 : FMT == KV_TQ3 ? 6 : FMT == KV_TQ2 ? 4 : 3;
+    const int at = bit & 31;
+    uint32_t c;                                        /* the codes times 128 */
+    if (at + NB > 32) c = __funnelshift_r(w[bit >> 5], w[(bit >> 5) + 1], at) << 7;
+    else c = at >= 7 ? w[bit >> 5] >> (at - 7) : w[bit >> 5] << (7 - at);
+    return attn_lut(c, ((1u << NB) - 1u) << 7, lane4);
+}
+
+/* K of a group as fragments: words of row g (lo) and row g + 8 (hi). `a`: the lane's address in the group's K. */
 template <int FMT, int HD>
-__device__ __forceinline__ void attn_k_words(const uint32_t* raw, uint32_t (&w)[HD / 8], uint32_t lane4) {
-    if constexpr (FMT == KV_RAW) {
+__device__ __forceinline__ void attn_load_k(uint32_t a, int t, uint32_t (&lo)[HD / 8], uint32_t (&hi)[HD / 8], uint32_t lane4) {
+    using F = AttnFmt<FMT, HD>;
+    if constexpr (F::MAT) {
+        constexpr int W = F::K_DIMS / 2;               /* halves' words of a word */
 #pragma unroll
-        for (int i = 0; i < HD / 8; i++) w[i] = raw[i];
-    } else if constexpr (!kv_is_tq(FMT)) {
+        for (int p = 0; p < F::PER_ROW / 2; p++) {     /* matrices: rows 0-7 and 8-15 of piece 2p, of piece 2p + 1 */
+            uint32_t w[4];
+            ldmatrix4(attn_pair<F::VEC>(a, p), attn_pair_at(p), w);
 #pragma unroll
-        for (int i = 0; i < HD / 16; i++) {
-            w[2 * i] = fp8_pair<FMT>(raw[i] & 0xffffu);
-            w[2 * i + 1] = fp8_pair<FMT>(raw[i] >> 16);
+            for (int k = 0; k < 2; k++) {
+                const int i = (2 * p + k) * W;
+                if constexpr (FMT == KV_RAW) {
+                    lo[i] = w[2 * k];
+                    hi[i] = w[2 * k + 1];
+                } else if constexpr (!kv_is_tq(FMT)) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        lo[i + x] = fp8_pair<FMT>(x ? w[2 * k] >> 16 : w[2 * k] & 0xffffu);
+                        hi[i + x] = fp8_pair<FMT>(x ? w[2 * k + 1] >> 16 : w[2 * k + 1] & 0xffffu);
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < W; x++) {
+                        lo[i + x] = attn_decode2<FMT>(&w[2 * k], 32 / W * x, lane4);
+                        hi[i + x] = attn_decode2<FMT>(&w[2 * k + 1], 32 / W * x, lane4);
+                    }
+                }
+            }
         }
     } else {
-        constexpr int NB = FMT == KV_TQ4 ? 8 : FMT == KV_TQ3 ? 6 : FMT == KV_TQ2 ? 4 : 3;     /* bits of two dims */
+        constexpr int N = FMT == KV_TQ3 ? 3 : 2, NB = FMT == KV_TQ3 ? 6 : 3;
+        uint32_t w[2][N + 1];
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+#pragma unroll
+            for (int n = 0; n < N; n++) w[r][n] = lds32(a, 8 * r * F::VEC + 4 * n);
+            if constexpr (FMT == KV_TQ1_5) {           /* the lane's 6 bytes begin in the middle of a word for odd t */
+                const int sh = (t & 1) * 16;
+                w[r][0] = __funnelshift_r(w[r][0], w[r][1], sh);
+                w[r][1] >>= sh;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const int bit = NB * i, at = bit & 31;
-            uint32_t c;                                /* the code pair times 128 */
-            if (at + NB > 32) c = (__funnelshift_r(raw[bit >> 5], raw[(bit >> 5) + 1], at) << 7);
-            else c = at >= 7 ? raw[bit >> 5] >> (at - 7) : raw[bit >> 5] << (7 - at);
-            w[i] = attn_lut(c, ((1u << NB) - 1u) << 7, lane4);
+            lo[i] = attn_decode2<FMT>(w[0], NB * i, lane4);
+            hi[i] = attn_decode2<FMT>(w[1], NB * i, lane4);
         }
     }
 }
-
-/* Two keys' V rows: x[e] = (key A, key B) at the lane's value e. */
+/* V of a group: xa[e] = keys (2t, 2t + 1), xc[e] = keys (2t + 8, 2t + 9) at the lane's value e. */
 template <int FMT, int HD>
-__device__ __forceinline__ void attn_v_pairs(const uint32_t* a, const uint32_t* b, uint32_t (&x)[HD / 8], uint32_t lane4) {
-    if constexpr (FMT == KV_RAW) {
+__device__ __forceinline__ void attn_load_v(uint32_t a, int g, uint32_t (&xa)[HD / 8], uint32_t (&xc)[HD / 8], uint32_t lane4) {
+    using F = AttnFmt<FMT, HD>;
+    if constexpr (F::MAT) {
 #pragma unroll
-        for (int i = 0; i < HD / 16; i++) {
-            x[2 * i] = __byte_perm(a[i], b[i], 0x5410);
-            x[2 * i + 1] = __byte_perm(a[i], b[i], 0x7632);
-        }
-    } else if constexpr (!kv_is_tq(FMT)) {
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) {
-            const uint32_t lo = __byte_perm(a[i], b[i], 0x5140), hi = __byte_perm(a[i], b[i], 0x7362);
-            x[4 * i] = fp8_pair<FMT>(lo & 0xffffu);
-            x[4 * i + 1] = fp8_pair<FMT>(lo >> 16);
-            x[4 * i + 2] = fp8_pair<FMT>(hi & 0xffffu);
-            x[4 * i + 3] = fp8_pair<FMT>(hi >> 16);
-        }
-    } else if constexpr (FMT == KV_TQ4) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t even = (a[i] & 0x0f0f0f0fu) | ((b[i] & 0x0f0f0f0fu) << 4);         /* dims 0, 2, 4, 6 of the eight */
-            const uint32_t odd = ((a[i] >> 4) & 0x0f0f0f0fu) | (b[i] & 0xf0f0f0f0u);
+        for (int p = 0; p < F::PER_ROW / 2; p++) {
+            uint32_t w[4];                             /* as K's, transposed: a word is (key 2t, key 2t + 1) */
+            ldmatrix4_trans(attn_pair<F::VEC>(a, p), attn_pair_at(p), w);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int s = 8 * k - 7;
-                x[8 * i + 2 * k] = attn_lut(s > 0 ? even >> s : even << -s, 0x7f80u, lane4);
-                x[8 * i + 2 * k + 1] = attn_lut(s > 0 ? odd >> s : odd << -s, 0x7f80u, lane4);
+                uint32_t(&x)[HD / 8] = (FMT == KV_RAW ? k >> 1 : k & 1) ? xc : xa;
+                const int c = 2 * p + (FMT == KV_RAW ? k & 1 : k >> 1);
+                if constexpr (FMT == KV_RAW) {
+                    x[c] = w[k];
+                } else if constexpr (!kv_is_tq(FMT)) {
+                    const uint32_t v = __byte_perm(w[k], 0, 0x3120);
+                    x[2 * c] = fp8_pair<FMT>(v & 0xffffu);
+                    x[2 * c + 1] = fp8_pair<FMT>(v >> 16);
+                } else if constexpr (FMT == KV_TQ4) {
+                    uint32_t even = w[k] & 0x0f0f0f0fu, odd = (w[k] >> 4) & 0x0f0f0f0fu;      /* A0 A2 B0 B2, A1 A3 B1 B3 */
+                    even |= even >> 12;                /* bytes 0, 1: A0 B0, A2 B2 */
+                    odd |= odd >> 12;
+                    x[4 * c] = attn_lut(even << 7, 0x7f80u, lane4);
+                    x[4 * c + 1] = attn_lut(odd << 7, 0x7f80u, lane4);
+                    x[4 * c + 2] = attn_lut(even >> 1, 0x7f80u, lane4);
+                    x[4 * c + 3] = attn_lut(odd >> 1, 0x7f80u, lane4);
+                } else {
+                    uint32_t even = w[k] & 0x33333333u, odd = (w[k] >> 2) & 0x33333333u;      /* every other code, A's in the low half */
+                    even |= even >> 14;                /* fields of 4 bits: A0 B0, A2 B2, .. */
+                    odd |= odd >> 14;
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        x[8 * c + 2 * y] = attn_lut(4 * y >= 7 ? even >> (4 * y - 7) : even << (7 - 4 * y), 0x780u, lane4);
+                        x[8 * c + 2 * y + 1] = attn_lut(4 * y >= 7 ? odd >> (4 * y - 7) : odd << (7 - 4 * y), 0x780u, lane4);
+                    }
+                }
             }
         }
     } else {
-        constexpr int W = FMT == KV_TQ2 ? 2 : 3;       /* bits of a code */
-        constexpr int N = FMT == KV_TQ1_5 ? 8 : 16;    /* codes of a lane's row; word 1 holds what word 0 does not */
+        constexpr int W = 3, N = FMT == KV_TQ1_5 ? 8 : 16;      /* codes of a lane's 24 or 48 bits of a row */
+        uint32_t w[4][2];
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            const int bit = W * e;
-            const uint32_t ca = (bit + W <= 32 ? a[0] >> bit : bit >= 32 ? a[1] >> (bit - 32) : __funnelshift_r(a[0], a[1], bit)) & ((1u << W) - 1u);
-            const uint32_t cb = (bit + W <= 32 ? b[0] >> bit : bit >= 32 ? b[1] >> (bit - 32) : __funnelshift_r(b[0], b[1], bit)) & ((1u << W) - 1u);
-            const uint32_t c = (ca | (cb << W)) << 7;
-            if constexpr (FMT == KV_TQ1_5) {
-                x[2 * e] = attn_lut(c, ~0u, lane4, 8 * 128);
-                x[2 * e + 1] = attn_lut(c, ~0u, lane4, (8 + 64) * 128);
-            } else {
-                x[e] = attn_lut(c, ~0u, lane4);
+        for (int r = 0; r < 4; r++) {
+            const int sh = 8 * (((FMT == KV_TQ3 ? 6 : 3) * g) & 3);
+            const uint32_t w0 = lds32(a, ((r & 1) + 8 * (r >> 1)) * F::VEC), w1 = lds32(a, ((r & 1) + 8 * (r >> 1)) * F::VEC + 4);
+            w[r][0] = __funnelshift_r(w0, w1, sh);
+            w[r][1] = w1 >> sh;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            uint32_t(&x)[HD / 8] = r ? xc : xa;
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const int bit = W * e;
+                uint32_t c[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    c[k] = (bit + W <= 32 ? w[r + k][0] >> bit : bit >= 32 ? w[r + k][1] >> (bit - 32) : __funnelshift_r(w[r + k][0], w[r + k][1], bit)) & 7u;
+                const uint32_t both = (c[0] | (c[1] << W)) << 7;
+                if constexpr (FMT == KV_TQ1_5) {
+                    x[2 * e] = attn_lut(both, ~0u, lane4, 8 * 128);
+                    x[2 * e + 1] = attn_lut(both, ~0u, lane4, (8 + 64) * 128);
+                } else {
+                    x[e] = attn_lut(both, ~0u, lane4);
+                }
             }
         }
     }
 }
+/* A lane's address in a group's K, and in its V, relative to their beginning. */
+template <int FMT, int HD> __device__ __forceinline__ uint32_t attn_k_at(int lane) {
+    using F = AttnFmt<FMT, HD>;
+    if (F::MAT) return attn_place<F::VEC>((lane & 7) + (lane & 8), lane >> 4);
+    return (lane >> 2) * F::VEC + (FMT == KV_TQ3 ? 12 * (lane & 3) : (6 * (lane & 3)) & ~3);
+}
+template <int FMT, int HD> __device__ __forceinline__ uint32_t attn_v_at(int lane) {
+    using F = AttnFmt<FMT, HD>;
+    if (FMT == KV_RAW) return attn_place<F::VEC>((lane & 7) + ((lane >> 4) << 3), (lane >> 3) & 1);      /* order of the product's operand */
+    if (F::MAT) return attn_place<F::VEC>((lane & 7) + (lane & 8), lane >> 4);
+    return 2 * (lane & 3) * F::VEC + (((FMT == KV_TQ3 ? 6 : 3) * (lane >> 2)) & ~3);
+}
 
-/* Where in a vector a lane's K and V bytes begin, unit n. */
-template <int FMT, int HD> __device__ __forceinline__ int attn_k_byte(int n, int t) {
-    if (FMT == KV_TQ3) return 12 * t + 4 * n;
-    if (FMT == KV_TQ2) return 8 * t;
-    if (FMT == KV_TQ1_5) return ((6 * t) & ~3) + 4 * n;
-    return 64 * n + 16 * t;                            /* TQ4: n = 0 */
-}
-template <int FMT, int HD> __device__ __forceinline__ int attn_v_byte(int n, int g) {
-    if (FMT == KV_TQ3) return ((6 * g) & ~3) + 4 * n;
-    if (FMT == KV_TQ2) return 4 * g;
-    if (FMT == KV_TQ1_5) return ((3 * g) & ~3) + (g < 7 ? 4 * n : 0);      /* the last lane's three bytes lie in one word */
-    return AttnFmt<FMT, HD>::VU == 16 ? 128 * n + 16 * g : 8 * g;
-}
-/* The odd start of a lane's bits in those words. */
-template <int FMT> __device__ __forceinline__ int attn_k_shift(int t) { return FMT == KV_TQ1_5 ? 8 * (6 * t - ((6 * t) & ~3)) : 0; }
-template <int FMT> __device__ __forceinline__ int attn_v_shift(int g) {
-    if (FMT == KV_TQ3) return 8 * ((6 * g) & 3);
-    if (FMT == KV_TQ1_5) return 8 * ((3 * g) & 3);
-    return 0;
+/* A lane's values 2 j and 2 j + 1 of a head's output. */
+template <int FMT> __device__ __forceinline__ void attn_store(__half* out, int j, int g, uint32_t two) {
+    if constexpr (FMT == KV_RAW) {
+        const __half2 h = *reinterpret_cast<const __half2*>(&two);
+        out[attn_v_dim<FMT>(2 * j, g)] = __low2half(h);
+        out[attn_v_dim<FMT>(2 * j + 1, g)] = __high2half(h);
+    } else {
+        *reinterpret_cast<uint32_t*>(out + attn_v_dim<FMT>(2 * j, g)) = two;
+    }
 }
 
 /* ---------------------------------------------------------------- work */
@@ -338,17 +406,6 @@ __device__ __forceinline__ int attn_keys(const AttnArgs& A, int b) {
 }
 __device__ __forceinline__ int attn_blocks(int n) { return (n + 63) >> kAttnPageShift; }
 __device__ __forceinline__ int attn_places(int n) { return n > 0 ? attn_blocks(n) + kAttnItemCost : 0; }
-/* f(0), f(1) .. f(N - 1) with the number as a type. */
-template <int N> struct AttnUnits {
-    template <typename Fn> static __device__ __forceinline__ void each(Fn&& f) {
-        AttnUnits<N - 1>::each(f);
-        f(std::integral_constant<int, N - 1>());
-    }
-};
-template <> struct AttnUnits<0> {
-    template <typename Fn> static __device__ __forceinline__ void each(Fn&&) {}
-};
-
 /* A place in the line of blocks: block blk of nb of item h (cache head x head block) of sequence b. */
 struct AttnAt {
     int b, h, hk, blk, nb, n, n_next;                  /* cache head hk; n keys here, n_next in sequence b + 1 */
@@ -475,14 +532,26 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         A.desc[part] = d;
     }
 
-    /* What is copied next. A lane's K rows are g, g + 8 of the warp's 16, its V rows 2t, 2t + 1, 2t + 8,
-     * 2t + 9; the pointers are those of its bytes in row 0 of the cache. */
+    /* What is copied next: units lane, lane + 32, .. of the group's rows. The pointers are those of the first
+     * of them in row 0 of the cache. */
     const uint32_t row_bytes = (uint32_t)A.n_kv * F::VEC;
     const uint8_t *klane, *vlane;
     int row_to;                                        /* cache row of the block's first position, -1: none; read one step ahead */
+    const uint32_t lane_off = (lane / F::PER_ROW) * row_bytes + (lane % F::PER_ROW) * F::UNIT;
+    auto copy_off = [&](int i) -> size_t {             /* of copy i beyond the lane's first */
+        if constexpr (32 % F::PER_ROW == 0) return (size_t)(i * (32 / F::PER_ROW)) * row_bytes;
+        else return (size_t)((32 * i + lane) / F::PER_ROW) * row_bytes + (32 * i + lane) % F::PER_ROW * F::UNIT - lane_off;
+    };
+    auto copy_row = [&](int i) -> int { return 32 % F::PER_ROW == 0 ? i * (32 / F::PER_ROW) + lane / F::PER_ROW : (32 * i + lane) / F::PER_ROW; };
+    /* where unit 32 i + lane goes: an exclusive or of the lane's first place with bits of i, or the same order */
+    const uint32_t lane_dst = F::MAT ? attn_place<F::VEC>(lane / F::PER_ROW, lane % F::PER_ROW) : lane * F::UNIT;
+    auto copy_dst = [](uint32_t d, int i) -> uint32_t {
+        constexpr int R = 32 / F::PER_ROW;             /* rows of a copy */
+        return F::MAT && F::VEC >= 128 ? d ^ (16u * ((i * R) & 7)) : d;
+    };
     auto aim_item = [&]() {
-        klane = A.k_store + (size_t)g * row_bytes + to.hk * F::VEC + attn_k_byte<FMT, HD>(0, t);
-        vlane = A.v_store + (size_t)(2 * t) * row_bytes + to.hk * F::VEC + attn_v_byte<FMT, HD>(0, g);
+        klane = A.k_store + to.hk * F::VEC + lane_off;
+        vlane = A.v_store + to.hk * F::VEC + lane_off;
     };
     auto aim = [&]() {
         if (A.block_table != nullptr) {
@@ -500,67 +569,48 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     auto issue = [&](int stage) -> int {               /* returns how many of the warp's 16 rows hold keys */
         int live = 0;
         if (to_places > 0) {
-            const uint32_t base = ring + stage * (32 * S::LANE_BYTES);
-            const uint32_t kd = base + lane * F::KU, vd = base + 32 * S::K_BYTES + lane * F::VU;
-            const uint32_t md = base + 32 * (S::K_BYTES + S::V_BYTES) + lane4;
+            const uint32_t base = ring + stage * S::STAGE, kd = base + lane_dst, md = base + 2 * S::ROWS + lane4;
             const int row0 = row_to + 16 * warp;
             live = row_to < 0 ? 0 : min(min(to.n - (to.blk << kAttnPageShift) - 16 * warp, A.n_slots - row0), 16);
             if (live == 16 && !(TQ && odd_end && row0 + 16 >= A.n_slots)) {
                 const uint8_t* kp = klane + (size_t)(uint32_t)row0 * row_bytes;
                 const uint8_t* vp = vlane + (size_t)(uint32_t)row0 * row_bytes;
-                AttnUnits<F::KN>::each([&](auto n) {
-                    constexpr int N = decltype(n)::value;
-                    const int off = attn_k_byte<FMT, HD>(N, t) - attn_k_byte<FMT, HD>(0, t);
-                    cp_async<F::KU, N * 32 * F::KU>(kd, kp + off);
-                    cp_async<F::KU, (F::KN + N) * 32 * F::KU>(kd, kp + 8 * (size_t)row_bytes + off);
-                });
-                AttnUnits<F::VN>::each([&](auto n) {
-                    constexpr int N = decltype(n)::value;
-                    const int off = attn_v_byte<FMT, HD>(N, g) - attn_v_byte<FMT, HD>(0, g);
-                    cp_async<F::VU, N * 32 * F::VU>(vd, vp + off);
-                    cp_async<F::VU, (F::VN + N) * 32 * F::VU>(vd, vp + row_bytes + off);
-                    cp_async<F::VU, (2 * F::VN + N) * 32 * F::VU>(vd, vp + 8 * (size_t)row_bytes + off);
-                    cp_async<F::VU, (3 * F::VN + N) * 32 * F::VU>(vd, vp + 9 * (size_t)row_bytes + off);
-                });
+#pragma unroll
+                for (int i = 0; i < F::COPIES; i++) {
+                    if (F::UNITS % 32 != 0 && 32 * i + lane >= F::UNITS) continue;
+                    cp_async<F::UNIT>(copy_dst(kd, i), 32 * F::UNIT * i, kp + copy_off(i));
+                    cp_async<F::UNIT>(copy_dst(kd, i), S::ROWS + 32 * F::UNIT * i, vp + copy_off(i));
+                }
                 if constexpr (TQ) {
                     /* the RMS values of rows g, g + 8: the 32-bit words that hold them */
                     const size_t at = (((size_t)(uint32_t)(row0 + g) * A.n_kv + to.hk) * 2) & ~(size_t)3;
                     const uint8_t* mk = reinterpret_cast<const uint8_t*>(A.k_meta) + at;
                     const uint8_t* mv = reinterpret_cast<const uint8_t*>(A.v_meta) + at;
-                    cp_async<4, 0>(md, mk);
-                    cp_async<4, 128>(md, mk + 16 * (size_t)A.n_kv);
-                    cp_async<4, 256>(md, mv);
-                    cp_async<4, 384>(md, mv + 16 * (size_t)A.n_kv);
+                    cp_async<4>(md, 0, mk);
+                    cp_async<4>(md, 128, mk + 16 * (size_t)A.n_kv);
+                    cp_async<4>(md, 256, mv);
+                    cp_async<4>(md, 384, mv + 16 * (size_t)A.n_kv);
                 }
             } else if (live > 0) {
                 /* rows behind the last key are filled with zeros, nothing of them is read */
                 const size_t first = (size_t)(uint32_t)row0 * row_bytes;
-                AttnUnits<F::KN>::each([&](auto n) {
-                    constexpr int N = decltype(n)::value;
-                    const int off = attn_k_byte<FMT, HD>(N, t) - attn_k_byte<FMT, HD>(0, t);
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const bool ok = g + 8 * r < live;
-                        const uint8_t* p = ok ? klane + first + 8 * r * (size_t)row_bytes + off : A.k_store;
-                        if (r == 0) cp_async_some<F::KU, N * 32 * F::KU>(kd, p, ok ? F::KU : 0);
-                        else cp_async_some<F::KU, (F::KN + N) * 32 * F::KU>(kd, p, ok ? F::KU : 0);
-                    }
-                });
-                AttnUnits<4 * F::VN>::each([&](auto n) {
-                    constexpr int N = decltype(n)::value % F::VN, R = decltype(n)::value / F::VN, KEY = (R & 1) + 8 * (R >> 1);
-                    const int off = attn_v_byte<FMT, HD>(N, g) - attn_v_byte<FMT, HD>(0, g);
-                    const bool ok = 2 * t + KEY < live;
-                    cp_async_some<F::VU, decltype(n)::value * 32 * F::VU>(vd, ok ? vlane + first + KEY * (size_t)row_bytes + off : A.v_store, ok ? F::VU : 0);
-                });
+                for (int i = 0; i < F::COPIES; i++) {
+                    if (F::UNITS % 32 != 0 && 32 * i + lane >= F::UNITS) continue;
+                    const bool ok = copy_row(i) < live;
+                    const size_t off = ok ? first + copy_off(i) : 0;
+                    cp_async_some<F::UNIT>(copy_dst(kd, i), 32 * F::UNIT * i, ok ? klane + off : A.k_store, ok ? F::UNIT : 0);
+                    cp_async_some<F::UNIT>(copy_dst(kd, i), S::ROWS + 32 * F::UNIT * i, ok ? vlane + off : A.v_store, ok ? F::UNIT : 0);
+                }
                 if constexpr (TQ) {
                     const size_t end = (size_t)A.n_slots * A.n_kv * 2;         /* bytes of an array */
-                    AttnUnits<4>::each([&](auto n) {
-                        constexpr int R = decltype(n)::value;
-                        const bool ok = g + 8 * (R & 1) < live;
-                        const size_t at = ok ? (((size_t)(uint32_t)(row0 + g + 8 * (R & 1)) * A.n_kv + to.hk) * 2) & ~(size_t)3 : 0;
-                        const uint8_t* p = reinterpret_cast<const uint8_t*>(R < 2 ? A.k_meta : A.v_meta) + at;
-                        cp_async_some<4, R * 128>(md, p, !ok ? 0 : at + 4 > end ? 2 : 4);
-                    });
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const bool ok = g + 8 * (r & 1) < live;
+                        const size_t at = ok ? (((size_t)(uint32_t)(row0 + g + 8 * (r & 1)) * A.n_kv + to.hk) * 2) & ~(size_t)3 : 0;
+                        const uint8_t* p = reinterpret_cast<const uint8_t*>(r < 2 ? A.k_meta : A.v_meta) + at;
+                        cp_async_some<4>(md, r * 128, p, !ok ? 0 : at + 4 > end ? 2 : 4);
+                    }
                 }
             }
             live = max(live, 0);
@@ -591,12 +641,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int n = 0; n < HD / 32; n++) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (8 * nt + g < heads)
-                    v = *reinterpret_cast<const uint4*>(src + (size_t)(8 * nt + g) * HD + attn_k_dim<FMT>(n, t));
-                q[nt][4 * n] = v.x; q[nt][4 * n + 1] = v.y; q[nt][4 * n + 2] = v.z; q[nt][4 * n + 3] = v.w;
-            }
+            for (int i = 0; i < HD / 8; i++)
+                q[nt][i] = 8 * nt + g < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)(8 * nt + g) * HD + attn_k_dim<FMT>(i, t)) : 0u;
     };
     float o[NT][TILES][4], m[NT][2], l[NT][2], vref;   /* m: the maximum less kWeightLog2 */
     auto begin_item = [&]() {
@@ -614,38 +660,22 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     load_q(at);
     begin_item();
 
+    const uint32_t k_at = attn_k_at<FMT, HD>(lane), v_at = attn_v_at<FMT, HD>(lane);
     int stage = 0;
     for (;;) {
         cp_wait<S::STAGES - 2>();
+        __syncwarp();                                  /* every lane's copies are there, and all have read the slot before */
         live_q[S::STAGES - 1] = issue(stage == 0 ? S::STAGES - 1 : stage - 1);     /* into the slot that the previous step emptied */
         const int live = live_q[0];
 #pragma unroll
         for (int s = 0; s + 1 < S::STAGES; s++) live_q[s] = live_q[s + 1];
-        const uint32_t base = ring + stage * (32 * S::LANE_BYTES);
-        const uint32_t kd = base + lane * F::KU, vd = base + 32 * S::K_BYTES + lane * F::VU;
+        const uint32_t base = ring + stage * S::STAGE;
         if (++stage == S::STAGES) stage = 0;
         float sk[2] = {1.0f, 1.0f}, sv[2] = {1.0f, 1.0f};
         float s[NT][4];
         if (live > 0) {                                /* uniform over the warp */
             uint32_t klo[HD / 8], khi[HD / 8];
-            {
-                uint32_t raw[2][F::KN * F::KU / 4 + 1];
-                AttnUnits<F::KN>::each([&](auto n) {
-                    constexpr int N = decltype(n)::value;
-                    lds_unit<F::KU, N * 32 * F::KU>(kd, &raw[0][N * (F::KU / 4)]);
-                    lds_unit<F::KU, (F::KN + N) * 32 * F::KU>(kd, &raw[1][N * (F::KU / 4)]);
-                });
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    if constexpr (FMT == KV_TQ1_5) {
-                        const int sh = attn_k_shift<FMT>(t);
-                        raw[r][0] = __funnelshift_r(raw[r][0], raw[r][1], sh);
-                        raw[r][1] >>= sh;
-                    }
-                }
-                attn_k_words<FMT, HD>(raw[0], klo, lane4);
-                attn_k_words<FMT, HD>(raw[1], khi, lane4);
-            }
+            attn_load_k<FMT, HD>(base + k_at, t, klo, khi, lane4);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -671,14 +701,14 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         }
         if (live > 0) {
             if constexpr (TQ) {
-                const uint32_t mb = base + 32 * (S::K_BYTES + S::V_BYTES) + lane4;
+                const uint32_t mb = base + 2 * S::ROWS + lane4;
                 /* which half of the word: the parity of the value's index (64 blk + 16 warp + 8 are even) */
                 const int bk = A.block_table != nullptr ? 0 : (int)(((long long)at.b * A.table_stride) & 1);
                 const int shift = (((bk + g) * A.n_kv + at.hk) & 1) * 16;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    sk[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb + 128 * r) >> shift)));
-                    sv[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb + 128 * (2 + r)) >> shift)));
+                    sk[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb, 128 * r) >> shift)));
+                    sv[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb, 128 * (2 + r)) >> shift)));
                 }
             }
             /* scores in base 2; rows behind the last key have none */
@@ -752,24 +782,8 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
                     bl[nt][r] = movmatrix(lo);
                 }
             {
-                uint32_t xa[HD / 8], xc[HD / 8];       /* keys (2t, 2t+1), (2t+8, 2t+9) */
-                {
-                    uint32_t raw[4][F::VN * F::VU / 4];
-                    AttnUnits<4 * F::VN>::each([&](auto n) {
-                        constexpr int N = decltype(n)::value;
-                        lds_unit<F::VU, N * 32 * F::VU>(vd, &raw[N / F::VN][N % F::VN * (F::VU / 4)]);
-                    });
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        if constexpr (FMT == KV_TQ3 || FMT == KV_TQ1_5) {
-                            const int sh = attn_v_shift<FMT>(g);
-                            raw[r][0] = __funnelshift_r(raw[r][0], raw[r][1], sh);
-                            raw[r][1] >>= sh;
-                        }
-                    }
-                    attn_v_pairs<FMT, HD>(raw[0], raw[1], xa, lane4);
-                    attn_v_pairs<FMT, HD>(raw[2], raw[3], xc, lane4);
-                }
+                uint32_t xa[HD / 8], xc[HD / 8];
+                attn_load_v<FMT, HD>(base + S::ROWS + v_at, g, xa, xc, lane4);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -869,9 +883,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const int h = 8 * nt + 2 * t + c;
-                        if (h < heads)
-                            *reinterpret_cast<uint32_t*>(A.out + (head0 + h) * HD + attn_v_dim<FMT, HD>(j, g)) =
-                                attn_out(acc[c], acc[c + 2], sum[nt][c]);
+                        if (h < heads) attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(acc[c], acc[c + 2], sum[nt][c]));
                     }
                 } else {
                     A.part_o[((size_t)slot * (NT * TILES) + x) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -949,7 +961,7 @@ __global__ void __launch_bounds__(kAttnJoinThreads) attn_join_kernel(const __gri
         for (int c = 0; c < 2; c++) {
             const int h = 8 * nt + 2 * t + c;
             if (h >= heads) continue;
-            *reinterpret_cast<uint32_t*>(A.out + (head0 + h) * HD + attn_v_dim<FMT, HD>(j, g)) = attn_out(a[c], a[c + 2], sum_s[2 * t + c]);
+            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(a[c], a[c + 2], sum_s[2 * t + c]));
         }
     }
     if (A.lse != nullptr && tid < 8 && 8 * nt + tid < heads)
