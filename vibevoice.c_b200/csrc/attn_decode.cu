@@ -170,9 +170,17 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-template <int FMT> __device__ __forceinline__ uint32_t fp8_pair(uint32_t two) {               /* two bytes -> two halves */
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, FMT == KV_E4M3 ? __NV_E4M3 : __NV_E5M2);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+/* Four FP8 values -> (0, 1) and (2, 3) as halves, or (SWAP) (0, 2) and (1, 3). An E5M2 byte is the upper half of
+ * its FP16 value, so a byte permute is the whole conversion. */
+template <int FMT, bool SWAP> __device__ __forceinline__ void fp8_halves(uint32_t w, uint32_t& a, uint32_t& b) {
+    if constexpr (FMT == KV_E5M2) {
+        a = __byte_perm(w, 0, SWAP ? 0x2404 : 0x1404);
+        b = __byte_perm(w, 0, SWAP ? 0x3414 : 0x3424);
+    } else {
+        if (SWAP) w = __byte_perm(w, 0, 0x3120);
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+            : "=r"(a), "=r"(b) : "r"(w));
+    }
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a, int at = 0) {
     uint32_t r;
@@ -268,11 +276,8 @@ __device__ __forceinline__ void attn_load_k(uint32_t a, int t, uint32_t (&lo)[HD
                     lo[i] = w[2 * k];
                     hi[i] = w[2 * k + 1];
                 } else if constexpr (!kv_is_tq(FMT)) {
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        lo[i + x] = fp8_pair<FMT>(x ? w[2 * k] >> 16 : w[2 * k] & 0xffffu);
-                        hi[i + x] = fp8_pair<FMT>(x ? w[2 * k + 1] >> 16 : w[2 * k + 1] & 0xffffu);
-                    }
+                    fp8_halves<FMT, false>(w[2 * k], lo[i], lo[i + 1]);
+                    fp8_halves<FMT, false>(w[2 * k + 1], hi[i], hi[i + 1]);
                 } else {
 #pragma unroll
                     for (int x = 0; x < W; x++) {
@@ -318,9 +323,7 @@ __device__ __forceinline__ void attn_load_v(uint32_t a, int g, uint32_t (&xa)[HD
                 if constexpr (FMT == KV_RAW) {
                     x[c] = w[k];
                 } else if constexpr (!kv_is_tq(FMT)) {
-                    const uint32_t v = __byte_perm(w[k], 0, 0x3120);
-                    x[2 * c] = fp8_pair<FMT>(v & 0xffffu);
-                    x[2 * c + 1] = fp8_pair<FMT>(v >> 16);
+                    fp8_halves<FMT, true>(w[k], x[2 * c], x[2 * c + 1]);
                 } else if constexpr (FMT == KV_TQ4) {
                     uint32_t even = w[k] & 0x0f0f0f0fu, odd = (w[k] >> 4) & 0x0f0f0f0fu;      /* A0 A2 B0 B2, A1 A3 B1 B3 */
                     even |= even >> 12;                /* bytes 0, 1: A0 B0, A2 B2 */
