@@ -60,9 +60,9 @@ constexpr int kAttnWarps = 4;                   /* a quarter of a 64-position bl
 #define VVB_ATTN_STAGES(FMT, HD, NT) (AttnFmt<FMT, HD>::VEC >= 256 ? 2 : kv_is_tq(FMT) ? 3 : 4)
 #endif
 constexpr int kAttnParts = VVB_ATTN_WAVES * 3 * 148;      /* parts the work is cut into, at most */
-constexpr int kAttnJoinCtas = 2 * 148;
+constexpr int kAttnFewItems = 37;               /* so many items, in eight tiles each, are one wave of the joining kernel */
+constexpr int kAttnJoinParts = 4, kAttnJoinChunk = 4;
 constexpr int kAttnItemCost = 1;                /* what beginning and ending an item costs, in blocks */
-constexpr int kAttnJoinThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kWeightLog2 = 12.0f;            /* a weight of 1 is kept as 2^12 ... */
 constexpr float kWeightTop = 15.0f;             /* ... and the maximum follows the scores once one passes 2^15 */
@@ -78,11 +78,12 @@ struct AttnArgs {
     const __half* v_meta;
     const int* block_table;    /* null: contiguous */
     const int* lens;
-    int2* desc;                /* [kAttnParts] item that ends in this CTA and began in an earlier one, that CTA; or -1 */
+    int2* desc;                /* cut items, see attn_join_kernel; -1: none. By item where there are few, else by part */
     float2* part_ml;           /* [2 kAttnParts][heads of an item] maximum, sum */
     float4* part_o;            /* [2 kAttnParts][tiles][32] output, in the lanes' layout */
     int n_seqs, n_q, n_kv, n_slots, table_stride, len_add;
     int group, head_blocks;    /* query heads to a cache head, items a cache head is cut into */
+    int by_item;
     float scale2;              /* scale * log2(e) */
 };
 
@@ -457,7 +458,6 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         for (int e = warp; e < F::LUT; e += kAttnWarps) *reinterpret_cast<uint32_t*>(attn_smem + 128 * e + lane4) = attn_lut_entry<FMT>(e);
     }
     pdl_wait();
-    pdl_trigger();
 
     /* This CTA's part of the line: sum the sequences' blocks, then find where the part begins. Each
      * item counts kAttnItemCost places more than it has blocks, ahead of its first block. */
@@ -503,6 +503,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         for (int i = tid; i < A.n_q * HD / 2; i += 32 * kAttnWarps) o[i] = 0;
         if (A.lse != nullptr)
             for (int i = tid; i < A.n_q; i += 32 * kAttnWarps) A.lse[(size_t)b * A.n_q + i] = -INFINITY;
+        if (A.by_item && tid < items) A.desc[b * items + tid] = make_int2(-1, 0);
     }
     __syncthreads();
 
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         places -= skipped;
     }
     if (places <= 0) {
-        if (tid == 0) A.desc[part] = make_int2(-1, 0);
+        if (tid == 0 && !A.by_item) A.desc[part] = make_int2(-1, 0);
         return;
     }
     at = to;
@@ -530,9 +531,10 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
             int p = (int)(first * parts / total);
             while (total * p / parts > first) p--;
             while (total * (p + 1) / parts <= first) p++;
-            d = make_int2(at.b * items + at.h, p);
+            d = make_int2(A.by_item ? part : at.b * items + at.h, p);
         }
-        A.desc[part] = d;
+        if (!A.by_item) A.desc[part] = d;
+        else if (d.x >= 0) A.desc[at.b * items + at.h] = d;
     }
 
     /* What is copied next: units lane, lane + 32, .. of the group's rows. The pointers are those of the first
@@ -813,6 +815,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         const size_t head0 = (size_t)at.b * A.n_q + (size_t)at.hk * A.group + h0;
         const bool whole = began && item_done;
         const int slot = 2 * part + (began ? 1 : 0);               /* an item that began here is this CTA's last */
+        if (A.by_item && whole && tid == 0) A.desc[at.b * items + at.h] = make_int2(-1, 0);
         float top[NT][2], sum[NT][2], f[NT][kAttnWarps][2];
 #pragma unroll
         for (int round = 0; round < S::ROUNDS; round++) {
@@ -902,74 +905,79 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     cp_wait<0>();
 }
 
-/* One CTA per part: the item that ends in the part and began in part `first` has its pieces in slots
- * 2 first + 1, 2 (first + 1), 2 (first + 2) .. 2 part. Warp w takes tile w % TILES of the output and
- * every (32 / TILES)-th piece. */
-template <int FMT, int HD, int NT>
-__global__ void __launch_bounds__(kAttnJoinThreads) attn_join_kernel(const __grid_constant__ AttnArgs A) {
-    constexpr int TILES = HD / 16, LANES = kAttnJoinThreads / 32 / TILES;
-    __shared__ float top_s[8], sum_s[8];
-    __shared__ float4 acc_s[kAttnJoinThreads / 32][32];
+/* Joins the pieces of items that are cut: an item that ends in part `last` and began in part `first` has them in
+ * slots 2 first + 1, 2 (first + 1), 2 (first + 2) .. 2 last. CTA (x, y) takes tile y of the output, of item x where
+ * there are few items (desc[item] = last, first), else of the items that end in parts 4 x .. 4 x + 3 (desc[last] =
+ * item, first). An item of up to four pieces is one warp's work, all its loads in flight at once; of a longer one
+ * each warp takes every WARPS-th piece and their results meet in shared memory. The order of every sum follows from
+ * the number of pieces alone. */
+struct AttnState {                                     /* a lane's: maximum and sum of heads 2t, 2t + 1, four outputs */
+    float m[2], l[2], o[4];
+    __device__ __forceinline__ void add(const float4& ml, const float4& v) {
+        const float m1[2] = {ml.x, ml.z}, l1[2] = {ml.y, ml.w}, v1[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const float top = fmaxf(m[c], m1[c]), a = ex2(m[c] - top), b = ex2(m1[c] - top);
+            m[c] = top;
+            l[c] = l[c] * a + l1[c] * b;
+            o[c] = o[c] * a + v1[c] * b;
+            o[c + 2] = o[c + 2] * a + v1[c + 2] * b;
+        }
+    }
+};
+template <int FMT, int HD, int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_constant__ AttnArgs A) {
+    constexpr int TILES = HD / 16;
+    __shared__ float4 ml_s[WARPS][32], o_s[WARPS][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int nt = blockIdx.y;
+    const int x = blockIdx.y, nt = x / TILES, j = x % TILES;
     pdl_wait();
-    pdl_trigger();
-    for (int part = blockIdx.x; part < kAttnParts; part += gridDim.x) {
-    const int2 d = A.desc[part];
-    if (d.x < 0) continue;
-    const int first = d.y, pieces = part - first + 1;
-    auto slot_of = [&](int p) { return p == 0 ? 2 * first + 1 : 2 * (first + p); };
-    if (warp < 8) {                                    /* head `warp` of the item */
-        float top = kNoMax;
-        for (int p = lane; p < pieces; p += 32) top = fmaxf(top, A.part_ml[(size_t)slot_of(p) * (8 * NT) + 8 * nt + warp].x);
+    const int per = A.by_item ? 1 : kAttnJoinParts, mine = blockIdx.x * per + lane;
+    int2 d = make_int2(-1, 0);
+    if (lane < per && (A.by_item || mine < kAttnParts)) d = A.desc[mine];
+    unsigned todo = __ballot_sync(0xffffffffu, d.x >= 0);
+    for (int n = 0; todo != 0; todo &= todo - 1) {
+        const int i = __ffs(todo) - 1, which = blockIdx.x * per + i;
+        const int dx = __shfl_sync(0xffffffffu, d.x, i), first = __shfl_sync(0xffffffffu, d.y, i);
+        const int item = A.by_item ? which : dx, pieces = (A.by_item ? dx : which) - first + 1;
+        const bool all = pieces > kAttnJoinChunk;
+        if (!all && (n++ % WARPS) != warp) continue;
+        AttnState s = {{kNoMax, kNoMax}, {0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        const int step = all ? WARPS : 1;
+        for (int p0 = all ? warp : 0; p0 < pieces; p0 += kAttnJoinChunk * step) {
+            float4 ml[kAttnJoinChunk], v[kAttnJoinChunk];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float sum = 0.0f;
-        for (int p = lane; p < pieces; p += 32) {
-            const float2 ml = A.part_ml[(size_t)slot_of(p) * (8 * NT) + 8 * nt + warp];
-            sum += ml.y * ex2(ml.x - top);
-        }
+            for (int k = 0; k < kAttnJoinChunk; k++) {
+                const int p = p0 + k * step;
+                if (p < pieces) {
+                    const size_t slot = p == 0 ? 2 * first + 1 : 2 * (first + p);
+                    ml[k] = *reinterpret_cast<const float4*>(A.part_ml + slot * (8 * NT) + 8 * nt + 2 * t);
+                    v[k] = A.part_o[(slot * (NT * TILES) + x) * 32 + lane];
+                }
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) { top_s[warp] = top; sum_s[warp] = sum; }
-    }
-    __syncthreads();
-    const int j = warp % TILES, sub = warp / TILES;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float top0 = top_s[2 * t], top1 = top_s[2 * t + 1];
-#pragma unroll 4
-    for (int p = sub; p < pieces; p += LANES) {
-        const size_t slot = slot_of(p);
-        const float4 v = A.part_o[(slot * (NT * TILES) + nt * TILES + j) * 32 + lane];
-        const float f0 = ex2(A.part_ml[slot * (8 * NT) + 8 * nt + 2 * t].x - top0);
-        const float f1 = ex2(A.part_ml[slot * (8 * NT) + 8 * nt + 2 * t + 1].x - top1);
-        acc.x = fmaf(v.x, f0, acc.x);
-        acc.y = fmaf(v.y, f1, acc.y);
-        acc.z = fmaf(v.z, f0, acc.z);
-        acc.w = fmaf(v.w, f1, acc.w);
-    }
-    acc_s[warp][lane] = acc;
-    __syncthreads();
-    const int items = A.n_kv * A.head_blocks;
-    const int b = d.x / items, item = d.x - b * items, hk = item / A.head_blocks, hb = item - hk * A.head_blocks;
-    const int heads = A.group - hb * 8 * NT;
-    const size_t head0 = (size_t)b * A.n_q + (size_t)hk * A.group + hb * 8 * NT;
-    if (sub == 0) {
-        for (int k = 1; k < LANES; k++) {
-            const float4 v = acc_s[warp + k * TILES][lane];
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            for (int k = 0; k < kAttnJoinChunk; k++)
+                if (p0 + k * step < pieces) s.add(ml[k], v[k]);
         }
-        const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+        if (all) {
+            __syncthreads();                           /* the previous long item has been read */
+            ml_s[warp][lane] = make_float4(s.m[0], s.l[0], s.m[1], s.l[1]);
+            o_s[warp][lane] = make_float4(s.o[0], s.o[1], s.o[2], s.o[3]);
+            __syncthreads();
+            if (warp != 0) continue;
+            for (int w = 1; w < WARPS; w++) s.add(ml_s[w][lane], o_s[w][lane]);
+        }
+        const int items = A.n_kv * A.head_blocks;
+        const int b = item / items, it = item - b * items, hk = it / A.head_blocks, hb = it - hk * A.head_blocks;
+        const int heads = A.group - hb * 8 * NT;
+        const size_t head0 = (size_t)b * A.n_q + (size_t)hk * A.group + hb * 8 * NT;
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             const int h = 8 * nt + 2 * t + c;
             if (h >= heads) continue;
-            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(a[c], a[c + 2], sum_s[2 * t + c]));
+            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(s.o[c], s.o[c + 2], s.l[c]));
+            if (A.lse != nullptr && j == 0 && g == 0) A.lse[head0 + h] = attn_lse(s.m[c], s.l[c]);
         }
-    }
-    if (A.lse != nullptr && tid < 8 && 8 * nt + tid < heads)
-        A.lse[head0 + 8 * nt + tid] = attn_lse(top_s[tid], sum_s[tid]);
-    __syncthreads();
     }
 }
 
@@ -992,9 +1000,19 @@ static cudaError_t launch_attn(const AttnArgs& A, cudaStream_t s) {
     constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM;
     cudaError_t e = cudaFuncSetAttribute((const void*)attn_decode_kernel<FMT, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(kAttnParts), dim3(32 * kAttnWarps), (size_t)SMEM, s, A);
+    /* Even parts want evenly filled SMs. A CTA that is placed while the kernel before still holds some of them
+     * starts where there is room, and its part ends late (64 x 4096: 107 us instead of 86, behind a kernel of 888
+     * small CTAs), so this is an ordinary launch unless there are few items: then the launch itself is what counts. */
+    if (A.by_item) {
+        e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(kAttnParts), dim3(32 * kAttnWarps), (size_t)SMEM, s, A);
+    } else {
+        attn_decode_kernel<FMT, HD, NT><<<dim3(kAttnParts), dim3(32 * kAttnWarps), (size_t)SMEM, s>>>(A);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attn_join_kernel<FMT, HD, NT>, dim3(kAttnJoinCtas, NT), dim3(kAttnJoinThreads), 0, s, A);
+    constexpr int TILES = NT * (HD / 16);
+    if (A.by_item) e = launch_pdl(attn_join_kernel<FMT, HD, NT, 8>, dim3(A.n_seqs * A.n_kv * A.head_blocks, TILES), dim3(256), 0, s, A);
+    else e = launch_pdl(attn_join_kernel<FMT, HD, NT, 4>, dim3((kAttnParts + kAttnJoinParts - 1) / kAttnJoinParts, TILES), dim3(128), 0, s, A);
     if (e == cudaSuccess) g_launches.fetch_add(2, std::memory_order_relaxed);
     return e;
 }
@@ -1028,7 +1046,8 @@ extern "C" int vvbk_attn_decode(const void* q, void* out, float* lse, const void
                         (const __half*)k_meta, (const __half*)v_meta, block_table, lens,
                         (int2*)base, (float2*)(base + sc.ml), (float4*)(base + sc.o),
                         n_seqs, n_q_heads, n_kv_heads, n_slots, table_stride, len_add,
-                        group, (group + 8 * nt - 1) / (8 * nt), scale * kLog2e};
+                        group, (group + 8 * nt - 1) / (8 * nt),
+                        (long long)n_seqs * n_kv_heads * ((group + 8 * nt - 1) / (8 * nt)) <= kAttnFewItems, scale * kLog2e};
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
     switch (kv_format) {
