@@ -55,9 +55,12 @@ constexpr int kAttnWarps = 4;                   /* a quarter of a 64-position bl
 #ifndef VVB_ATTN_WAVES
 #define VVB_ATTN_WAVES 1
 #endif
+#ifndef VVB_ATTN_KG
+#define VVB_ATTN_KG (VEC >= 256 ? 1 : 2)
+#endif
 #ifndef VVB_ATTN_CTAS
 #define VVB_ATTN_CTAS(FMT, HD, NT) (HD == 256 || NT == 2 ? 2 : 3)
-#define VVB_ATTN_STAGES(FMT, HD, NT) (AttnFmt<FMT, HD>::VEC >= 256 ? 2 : kv_is_tq(FMT) ? 3 : 4)
+#define VVB_ATTN_STAGES(FMT, HD, NT) (FMT == KV_TQ4 || AttnFmt<FMT, HD>::VEC * AttnFmt<FMT, HD>::KG >= 256 ? 2 : 3)
 #endif
 constexpr int kAttnParts = VVB_ATTN_WAVES * 3 * 148;      /* parts the work is cut into, at most */
 constexpr int kAttnFewItems = 37;               /* so many items, in eight tiles each, are one wave of the joining kernel */
@@ -96,7 +99,9 @@ template <int FMT, int HD> struct AttnFmt {
     static constexpr int VEC = kv_is_tq(FMT) ? tq_bytes_per_vec(FMT) : FMT == KV_RAW ? 2 * HD : HD;
     static constexpr bool MAT = FMT != KV_TQ3 && FMT != KV_TQ1_5;
     static constexpr int UNIT = FMT == KV_TQ1_5 ? 8 : 16;
-    static constexpr int PER_ROW = VEC / UNIT, UNITS = 16 * PER_ROW, COPIES = (UNITS + 31) / 32;      /* of a group, copies a lane makes */
+    static constexpr int KG = VVB_ATTN_KG;                       /* groups a warp takes in a step; the four warps' groups are a block */
+    static constexpr int KEYS = 16 * KG, BLOCK = 4 * KEYS;
+    static constexpr int PER_ROW = VEC / UNIT, UNITS = KEYS * PER_ROW, COPIES = (UNITS + 31) / 32;    /* of a step, copies a lane makes */
     /* dims of a word that ldmatrix brings: of K a lane's 4 bytes, of V the 2 bytes of one key */
     static constexpr int K_DIMS = FMT == KV_RAW ? 2 : FMT == KV_TQ4 ? 8 : FMT == KV_TQ2 ? 16 : 4;
     /* entries of the code table: two codes -> two levels; 1.5 bits: code -> pair, then two keys' codes -> two pairs */
@@ -110,8 +115,8 @@ template <int FMT> __host__ __device__ constexpr float attn_alpha() {
 
 template <int FMT, int HD, int NT> struct AttnShape {
     using F = AttnFmt<FMT, HD>;
-    static constexpr int ROWS = 16 * F::VEC;                                                  /* bytes of a group's K, or V */
-    static constexpr int STAGE = 2 * ROWS + (kv_is_tq(FMT) ? 512 : 0);                        /* then its RMS values, a lane's own words */
+    static constexpr int GROUP = 16 * F::VEC, ROWS = F::KG * GROUP;                           /* bytes of a group's K, or V; of a step's */
+    static constexpr int STAGE = 2 * ROWS + (kv_is_tq(FMT) ? 8 * F::KEYS : 0);                /* then the words that hold the rows' RMS values */
     static constexpr int CTAS = VVB_ATTN_CTAS(FMT, HD, NT);                                   /* an SM's, by registers and shared memory */
     static constexpr int STAGES = VVB_ATTN_STAGES(FMT, HD, NT);
     static constexpr int RING = STAGE * STAGES;                                               /* a warp's */
@@ -406,12 +411,12 @@ template <int FMT> __device__ __forceinline__ void attn_store(__half* out, int j
 __device__ __forceinline__ int attn_keys(const AttnArgs& A, int b) {
     const long long cap = A.block_table != nullptr ? (long long)A.table_stride << kAttnPageShift : (long long)A.table_stride;
     const long long n = (long long)__ldg(A.lens + b) + A.len_add;
-    return (int)min(min(max(n, 0ll), cap), 0x7fffffc0ll);
+    return (int)min(min(max(n, 0ll), cap), 0x7fffff00ll);
 }
-__device__ __forceinline__ int attn_blocks(int n) { return (n + 63) >> kAttnPageShift; }
-__device__ __forceinline__ int attn_places(int n) { return n > 0 ? attn_blocks(n) + kAttnItemCost : 0; }
+template <int BLOCK> __device__ __forceinline__ int attn_blocks(int n) { return (int)(((unsigned)n + (BLOCK - 1)) / BLOCK); }
+template <int BLOCK> __device__ __forceinline__ int attn_places(int n) { return n > 0 ? attn_blocks<BLOCK>(n) + kAttnItemCost : 0; }
 /* A place in the line of blocks: block blk of nb of item h (cache head x head block) of sequence b. */
-struct AttnAt {
+template <int BLOCK> struct AttnAt {
     int b, h, hk, blk, nb, n, n_next;                  /* cache head hk; n keys here, n_next in sequence b + 1 */
     __device__ __forceinline__ void set(const AttnArgs& A, int seq, int item, int block) {
         b = seq;
@@ -419,7 +424,7 @@ struct AttnAt {
         hk = h / A.head_blocks;
         blk = block;
         n = attn_keys(A, b);
-        nb = attn_blocks(n);
+        nb = attn_blocks<BLOCK>(n);
         n_next = b + 1 < A.n_seqs ? attn_keys(A, b + 1) : 0;
     }
     __device__ __forceinline__ bool last() const { return blk + 1 >= nb; }                    /* of the item */
@@ -435,7 +440,7 @@ struct AttnAt {
             n = n_next;
             n_next = b + 1 < A.n_seqs ? attn_keys(A, b + 1) : 0;
         } while (n == 0 && b < A.n_seqs);
-        nb = attn_blocks(n);
+        nb = attn_blocks<BLOCK>(n);
     }
 };
 
@@ -465,7 +470,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     const int per = (A.n_seqs + 32 * kAttnWarps - 1) / (32 * kAttnWarps);
     const int s0 = min(tid * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
     long long mine = 0;
-    for (int b = s0; b < s1; b++) mine += attn_places(attn_keys(A, b));
+    for (int b = s0; b < s1; b++) mine += attn_places<F::BLOCK>(attn_keys(A, b));
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     if (u0 < u1 && mine > 0 && u0 >= before * items && u0 < (before + mine) * items) {
         long long at = before;                         /* one thread finds itself here */
         for (int b = s0; b < s1; b++) {
-            const int np = attn_places(attn_keys(A, b));
+            const int np = attn_places<F::BLOCK>(attn_keys(A, b));
             if (u0 < (at + np) * items) {
                 find_s = b;
                 scan_s[kAttnWarps] = u0 - at * items;
@@ -507,11 +512,11 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     }
     __syncthreads();
 
-    AttnAt to, at;                                     /* what is copied next, what is computed next */
+    AttnAt<F::BLOCK> to, at;                                     /* what is copied next, what is computed next */
     int places = (int)(u1 - u0), skipped = 0;          /* of the line that are left to this CTA */
     if (places > 0) {
         const long long in = scan_s[kAttnWarps];
-        const int b = find_s, np = attn_places(attn_keys(A, b)), item = (int)(in / np);
+        const int b = find_s, np = attn_places<F::BLOCK>(attn_keys(A, b)), item = (int)(in / np);
         const int off = (int)(in - (long long)item * np);
         to.set(A, b, item, max(off - kAttnItemCost, 0));
         skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
@@ -541,7 +546,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
      * of them in row 0 of the cache. */
     const uint32_t row_bytes = (uint32_t)A.n_kv * F::VEC;
     const uint8_t *klane, *vlane;
-    int row_to;                                        /* cache row of the block's first position, -1: none; read one step ahead */
+    int row_to;                                        /* cache row of the warp's first key, -1: none; read one step ahead */
     const uint32_t lane_off = (lane / F::PER_ROW) * row_bytes + (lane % F::PER_ROW) * F::UNIT;
     auto copy_off = [&](int i) -> size_t {             /* of copy i beyond the lane's first */
         if constexpr (32 % F::PER_ROW == 0) return (size_t)(i * (32 / F::PER_ROW)) * row_bytes;
@@ -558,13 +563,17 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         klane = A.k_store + to.hk * F::VEC + lane_off;
         vlane = A.v_store + to.hk * F::VEC + lane_off;
     };
-    auto aim = [&]() {
-        if (A.block_table != nullptr) {
-            const int page = __ldg(A.block_table + (size_t)to.b * A.table_stride + to.blk);
-            row_to = (unsigned)page <= (unsigned)(A.n_slots - 1) >> kAttnPageShift ? page << kAttnPageShift : -1;
-        } else {
-            const long long row = (long long)to.b * A.table_stride + ((long long)to.blk << kAttnPageShift);
-            row_to = row < A.n_slots ? (int)row : -1;
+    auto aim = [&]() {                                 /* this warp's rows of block to.blk: never across a page */
+        const int at = to.blk * F::BLOCK + F::KEYS * warp;
+        row_to = -1;
+        if (at < to.n) {
+            if (A.block_table != nullptr) {
+                const int page = __ldg(A.block_table + (size_t)to.b * A.table_stride + (at >> kAttnPageShift));
+                if ((unsigned)page <= (unsigned)(A.n_slots - 1) >> kAttnPageShift) row_to = (page << kAttnPageShift) + (at & 63);
+            } else {
+                const long long row = (long long)to.b * A.table_stride + at;
+                if (row < A.n_slots) row_to = (int)row;
+            }
         }
     };
     aim_item();
@@ -575,9 +584,9 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         int live = 0;
         if (to_places > 0) {
             const uint32_t base = ring + stage * S::STAGE, kd = base + lane_dst, md = base + 2 * S::ROWS + lane4;
-            const int row0 = row_to + 16 * warp;
-            live = row_to < 0 ? 0 : min(min(to.n - (to.blk << kAttnPageShift) - 16 * warp, A.n_slots - row0), 16);
-            if (live == 16 && !(TQ && odd_end && row0 + 16 >= A.n_slots)) {
+            const int row0 = row_to;
+            live = row_to < 0 ? 0 : min(min(to.n - to.blk * F::BLOCK - F::KEYS * warp, A.n_slots - row0), F::KEYS);
+            if (live == F::KEYS && !(TQ && odd_end && row0 + F::KEYS >= A.n_slots)) {
                 const uint8_t* kp = klane + (size_t)(uint32_t)row0 * row_bytes;
                 const uint8_t* vp = vlane + (size_t)(uint32_t)row0 * row_bytes;
 #pragma unroll
@@ -587,14 +596,13 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
                     cp_async<F::UNIT>(copy_dst(kd, i), S::ROWS + 32 * F::UNIT * i, vp + copy_off(i));
                 }
                 if constexpr (TQ) {
-                    /* the RMS values of rows g, g + 8: the 32-bit words that hold them */
-                    const size_t at = (((size_t)(uint32_t)(row0 + g) * A.n_kv + to.hk) * 2) & ~(size_t)3;
-                    const uint8_t* mk = reinterpret_cast<const uint8_t*>(A.k_meta) + at;
-                    const uint8_t* mv = reinterpret_cast<const uint8_t*>(A.v_meta) + at;
-                    cp_async<4>(md, 0, mk);
-                    cp_async<4>(md, 128, mk + 16 * (size_t)A.n_kv);
-                    cp_async<4>(md, 256, mv);
-                    cp_async<4>(md, 384, mv + 16 * (size_t)A.n_kv);
+                    /* the RMS values: for each row the 32-bit word that holds it, K's rows, then V's */
+#pragma unroll
+                    for (int i = 0; i < F::KG; i++) {
+                        const int w = 32 * i + lane;
+                        const size_t at = (((size_t)(uint32_t)(row0 + w % F::KEYS) * A.n_kv + to.hk) * 2) & ~(size_t)3;
+                        cp_async<4>(md, 128 * i, reinterpret_cast<const uint8_t*>(w < F::KEYS ? A.k_meta : A.v_meta) + at);
+                    }
                 }
             } else if (live > 0) {
                 /* rows behind the last key are filled with zeros, nothing of them is read */
@@ -610,11 +618,11 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
                 if constexpr (TQ) {
                     const size_t end = (size_t)A.n_slots * A.n_kv * 2;         /* bytes of an array */
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const bool ok = g + 8 * (r & 1) < live;
-                        const size_t at = ok ? (((size_t)(uint32_t)(row0 + g + 8 * (r & 1)) * A.n_kv + to.hk) * 2) & ~(size_t)3 : 0;
-                        const uint8_t* p = reinterpret_cast<const uint8_t*>(r < 2 ? A.k_meta : A.v_meta) + at;
-                        cp_async_some<4>(md, r * 128, p, !ok ? 0 : at + 4 > end ? 2 : 4);
+                    for (int i = 0; i < F::KG; i++) {
+                        const int w = 32 * i + lane, row = w % F::KEYS;
+                        const bool ok = row < live;
+                        const size_t at = ok ? (((size_t)(uint32_t)(row0 + row) * A.n_kv + to.hk) * 2) & ~(size_t)3 : 0;
+                        cp_async_some<4>(md, 128 * i, reinterpret_cast<const uint8_t*>(w < F::KEYS ? A.k_meta : A.v_meta) + at, !ok ? 0 : at + 4 > end ? 2 : 4);
                     }
                 }
             }
@@ -640,7 +648,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     for (int s = 0; s < S::STAGES - 1; s++) live_q[s] = issue(s);
 
     uint32_t q[NT][HD / 8];
-    auto load_q = [&](const AttnAt& x) {
+    auto load_q = [&](const AttnAt<F::BLOCK>& x) {
         const int h0 = (x.h - x.hk * A.head_blocks) * 8 * NT, heads = A.group - h0;      /* of this block: at most 8 NT */
         const __half* src = A.q + ((size_t)x.b * A.n_q + (size_t)x.hk * A.group + h0) * HD;
 #pragma unroll
@@ -676,28 +684,30 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         for (int s = 0; s + 1 < S::STAGES; s++) live_q[s] = live_q[s + 1];
         const uint32_t base = ring + stage * S::STAGE;
         if (++stage == S::STAGES) stage = 0;
-        float sk[2] = {1.0f, 1.0f}, sv[2] = {1.0f, 1.0f};
-        float s[NT][4];
+        float s[F::KG][NT][4];
         if (live > 0) {                                /* uniform over the warp */
-            uint32_t klo[HD / 8], khi[HD / 8];
-            attn_load_k<FMT, HD>(base + k_at, t, klo, khi, lane4);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int gi = 0; gi < F::KG; gi++) {
+                uint32_t klo[HD / 8], khi[HD / 8];
+                attn_load_k<FMT, HD>(base + gi * S::GROUP + k_at, t, klo, khi, lane4);
 #pragma unroll
-                for (int ks = 0; ks < HD / 16; ks += 2) {
-                    mma16816(s0, klo[2 * ks], khi[2 * ks], klo[2 * ks + 1], khi[2 * ks + 1], q[nt][2 * ks], q[nt][2 * ks + 1]);
-                    mma16816(s1, klo[2 * ks + 2], khi[2 * ks + 2], klo[2 * ks + 3], khi[2 * ks + 3], q[nt][2 * ks + 2], q[nt][2 * ks + 3]);
+                for (int nt = 0; nt < NT; nt++) {
+                    float s0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ks += 2) {
+                        mma16816(s0, klo[2 * ks], khi[2 * ks], klo[2 * ks + 1], khi[2 * ks + 1], q[nt][2 * ks], q[nt][2 * ks + 1]);
+                        mma16816(s1, klo[2 * ks + 2], khi[2 * ks + 2], klo[2 * ks + 3], khi[2 * ks + 3], q[nt][2 * ks + 2], q[nt][2 * ks + 3]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s[gi][nt][c] = s0[c] + s1[c];
                 }
-#pragma unroll
-                for (int c = 0; c < 4; c++) s[nt][c] = s0[c] + s1[c];
             }
         }
         /* the next item's Q is on its way while this one is finished */
         const bool item_done = at.last();
         places--;
         const bool more = item_done ? places > kAttnItemCost : places > 0;
-        AttnAt nx = at;
+        AttnAt<F::BLOCK> nx = at;
         if (!item_done) {
             nx.blk++;
         } else if (more) {
@@ -705,40 +715,55 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
             load_q(nx);
         }
         if (live > 0) {
+            float sv[F::KG][2], sv_top = 0.0f;
             if constexpr (TQ) {
-                const uint32_t mb = base + 2 * S::ROWS + lane4;
-                /* which half of the word: the parity of the value's index (64 blk + 16 warp + 8 are even) */
+                const uint32_t mb = base + 2 * S::ROWS + 4 * g;
+                /* which half of the word: the parity of the value's index (a warp's first position is even, and so is 8) */
                 const int bk = A.block_table != nullptr ? 0 : (int)(((long long)at.b * A.table_stride) & 1);
                 const int shift = (((bk + g) * A.n_kv + at.hk) & 1) * 16;
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    sk[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb, 128 * r) >> shift)));
-                    sv[r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb, 128 * (2 + r)) >> shift)));
-                }
+                for (int gi = 0; gi < F::KG; gi++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const float sk = __half2float(__ushort_as_half((unsigned short)(lds32(mb, 64 * gi + 32 * r) >> shift)));
+                        const float f = A.scale2 * (sk * (1.0f / attn_alpha<FMT>()));
+                        sv[gi][r] = __half2float(__ushort_as_half((unsigned short)(lds32(mb, 64 * F::KG + 64 * gi + 32 * r) >> shift)));
+                        sv_top = fmaxf(sv_top, sv[gi][r]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int c = 0; c < 2; c++) s[gi][nt][2 * r + c] *= f;
+                    }
+            } else {
+#pragma unroll
+                for (int gi = 0; gi < F::KG; gi++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) s[gi][nt][c] *= A.scale2;
             }
             /* scores in base 2; rows behind the last key have none */
+            if (live < F::KEYS) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int gi = 0; gi < F::KG; gi++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) s[nt][c] *= TQ ? A.scale2 * (sk[c >> 1] * (1.0f / attn_alpha<FMT>())) : A.scale2;
-            if (live < 16) {
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            if (16 * gi + g + 8 * (c >> 1) >= live) s[gi][nt][c] = -INFINITY;
+            }
+            bool up = TQ && sv_top > vref;
+#pragma unroll
+            for (int gi = 0; gi < F::KG; gi++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        if (g + 8 * (c >> 1) >= live) s[nt][c] = -INFINITY;
-            }
-            bool up = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) up |= s[nt][c] > m[nt][c & 1] + kWeightTop;
-            if constexpr (TQ) up |= fmaxf(sv[0], sv[1]) > vref;
+                    for (int c = 0; c < 4; c++) up |= s[gi][nt][c] > m[nt][c & 1] + kWeightTop;
             if (__any_sync(0xffffffffu, up)) {
                 /* a new maximum (or a larger RMS of V): rescale what there is */
                 float rv = 1.0f;
                 if constexpr (TQ) {
-                    float x = fmaxf(sv[0], sv[1]);
+                    float x = sv_top;
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     if (x > vref) {                    /* the next power of two above it */
@@ -751,7 +776,9 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        float x = fmaxf(s[nt][c], s[nt][c + 2]);
+                        float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+                        for (int gi = 1; gi < F::KG; gi++) x = fmaxf(x, fmaxf(s[gi][nt][c], s[gi][nt][c + 2]));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -766,29 +793,30 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
                         }
                     }
             }
-            /* weights: FP32 sums, FP16 pairs for the product */
-            uint32_t bh[NT][2], bl[NT][2];
             const float inv = 1.0f / vref;             /* (a power of two) */
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int gi = 0; gi < F::KG; gi++) {
+                /* weights: FP32 sums, FP16 pairs for the product */
+                uint32_t bh[NT][2], bl[NT][2];
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    float w[2];
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        w[c] = ex2(s[nt][2 * r + c] - m[nt][c]);
-                        l[nt][c] += w[c];
-                        if constexpr (TQ) w[c] *= sv[r] * inv;
+                    for (int r = 0; r < 2; r++) {
+                        float w[2];
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            w[c] = ex2(s[gi][nt][2 * r + c] - m[nt][c]);
+                            l[nt][c] += w[c];
+                            if constexpr (TQ) w[c] *= sv[gi][r] * inv;
+                        }
+                        const uint32_t hi = pack2_rz(w[0], w[1]);
+                        const float2 h = unpack2(hi);
+                        const uint32_t lo = hmax2_bits(pack2(w[0] - h.x, w[1] - h.y), 0x00010001u);      /* at least 2^-24 */
+                        bh[nt][r] = movmatrix(hi);
+                        bl[nt][r] = movmatrix(lo);
                     }
-                    const uint32_t hi = pack2_rz(w[0], w[1]);
-                    const float2 h = unpack2(hi);
-                    const uint32_t lo = hmax2_bits(pack2(w[0] - h.x, w[1] - h.y), 0x00010001u);      /* at least 2^-24 */
-                    bh[nt][r] = movmatrix(hi);
-                    bl[nt][r] = movmatrix(lo);
-                }
-            {
                 uint32_t xa[HD / 8], xc[HD / 8];
-                attn_load_v<FMT, HD>(base + S::ROWS + v_at, g, xa, xc, lane4);
+                attn_load_v<FMT, HD>(base + S::ROWS + gi * S::GROUP + v_at, g, xa, xc, lane4);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
