@@ -51,18 +51,17 @@ namespace vvb {
 extern std::atomic<uint64_t> g_launches;
 
 constexpr int kAttnPageShift = 6;
-constexpr int kAttnWarps = 4;                   /* a quarter of a 64-position block each */
-#ifndef VVB_ATTN_WAVES
-#define VVB_ATTN_WAVES 1
-#endif
 #ifndef VVB_ATTN_KG
-#define VVB_ATTN_KG (VEC >= 256 ? 1 : 2)
+#define VVB_ATTN_KG (VEC >= 256 ? 1 : VEC >= 64 ? 2 : 4)
+#endif
+#ifndef VVB_ATTN_WARPS
+#define VVB_ATTN_WARPS(FMT, HD) 4
 #endif
 #ifndef VVB_ATTN_CTAS
 #define VVB_ATTN_CTAS(FMT, HD, NT) (HD == 256 || NT == 2 ? 2 : 3)
 #define VVB_ATTN_STAGES(FMT, HD, NT) (FMT == KV_TQ4 || AttnFmt<FMT, HD>::VEC * AttnFmt<FMT, HD>::KG >= 256 ? 2 : 3)
 #endif
-constexpr int kAttnParts = VVB_ATTN_WAVES * 3 * 148;      /* parts the work is cut into, at most */
+constexpr int kAttnSms = 148, kAttnParts = 3 * kAttnSms;      /* parts the work is cut into, at most */
 constexpr int kAttnFewItems = 37;               /* so many items, in eight tiles each, are one wave of the joining kernel */
 constexpr int kAttnJoinParts = 4, kAttnJoinChunk = 4;
 constexpr int kAttnItemCost = 1;                /* what beginning and ending an item costs, in blocks */
@@ -86,6 +85,7 @@ struct AttnArgs {
     float4* part_o;            /* [2 kAttnParts][tiles][32] output, in the lanes' layout */
     int n_seqs, n_q, n_kv, n_slots, table_stride, len_add;
     int group, head_blocks;    /* query heads to a cache head, items a cache head is cut into */
+    int parts;                 /* CTAs of the launch */
     int by_item;
     float scale2;              /* scale * log2(e) */
 };
@@ -99,8 +99,9 @@ template <int FMT, int HD> struct AttnFmt {
     static constexpr int VEC = kv_is_tq(FMT) ? tq_bytes_per_vec(FMT) : FMT == KV_RAW ? 2 * HD : HD;
     static constexpr bool MAT = FMT != KV_TQ3 && FMT != KV_TQ1_5;
     static constexpr int UNIT = FMT == KV_TQ1_5 ? 8 : 16;
-    static constexpr int KG = VVB_ATTN_KG;                       /* groups a warp takes in a step; the four warps' groups are a block */
-    static constexpr int KEYS = 16 * KG, BLOCK = 4 * KEYS;
+    static constexpr int KG = VVB_ATTN_KG;                       /* groups a warp takes in a step; the warps' groups are a block */
+    static constexpr int W = VVB_ATTN_WARPS(FMT, HD);            /* warps of a CTA */
+    static constexpr int KEYS = 16 * KG, BLOCK = W * KEYS;
     static constexpr int PER_ROW = VEC / UNIT, UNITS = KEYS * PER_ROW, COPIES = (UNITS + 31) / 32;    /* of a step, copies a lane makes */
     /* dims of a word that ldmatrix brings: of K a lane's 4 bytes, of V the 2 bytes of one key */
     static constexpr int K_DIMS = FMT == KV_RAW ? 2 : FMT == KV_TQ4 ? 8 : FMT == KV_TQ2 ? 16 : 4;
@@ -116,16 +117,16 @@ template <int FMT> __host__ __device__ constexpr float attn_alpha() {
 template <int FMT, int HD, int NT> struct AttnShape {
     using F = AttnFmt<FMT, HD>;
     static constexpr int GROUP = 16 * F::VEC, ROWS = F::KG * GROUP;                           /* bytes of a group's K, or V; of a step's */
-    static constexpr int STAGE = 2 * ROWS + (kv_is_tq(FMT) ? 8 * F::KEYS : 0);                /* then the words that hold the rows' RMS values */
+    static constexpr int USED = 2 * ROWS + (kv_is_tq(FMT) ? 8 * F::KEYS : 0);                 /* then the words that hold the rows' RMS values */
+    static constexpr int OUT = NT * HD * 32;                                                  /* a warp's output, left in the stage it has read last */
+    static constexpr int STAGE = USED > OUT ? USED : OUT;
     static constexpr int CTAS = VVB_ATTN_CTAS(FMT, HD, NT);                                   /* an SM's, by registers and shared memory */
     static constexpr int STAGES = VVB_ATTN_STAGES(FMT, HD, NT);
     static constexpr int RING = STAGE * STAGES;                                               /* a warp's */
     static constexpr int TILES = HD / 16;                                                     /* 16-dim tiles of the output */
-    static constexpr int MINE = NT * TILES / kAttnWarps;                                      /* of them a warp finishes, ... */
-    static constexpr int PER_ROUND = 1, ROUNDS = MINE / PER_ROUND;                            /* ... so many in one round of the exchange */
-    static constexpr int XCHG = kAttnWarps * (kAttnWarps - 1) * PER_ROUND * 32 * 16;
+    static constexpr int MINE = NT * TILES / F::W;                                            /* of them a warp finishes */
     static constexpr int LUT = F::LUT * 128;
-    static constexpr int SMEM = LUT + kAttnWarps * RING + XCHG;       /* in this order */
+    static constexpr int SMEM = LUT + F::W * RING;                                            /* in this order */
 };
 
 /* ---------------------------------------------------------------- instructions */
@@ -445,29 +446,28 @@ template <int BLOCK> struct AttnAt {
 };
 
 template <int FMT, int HD, int NT>
-__global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, NT>::CTAS) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
     using F = AttnFmt<FMT, HD>;
     using S = AttnShape<FMT, HD, NT>;
     constexpr bool TQ = kv_is_tq(FMT);
-    constexpr int TILES = S::TILES, MINE = S::MINE;    /* tiles of the output, those a warp finishes */
-    __shared__ float m_s[kAttnWarps][8 * NT], l_s[kAttnWarps][8 * NT], f_s[kAttnWarps];
-    __shared__ long long scan_s[kAttnWarps + 1];
+    constexpr int W = F::W, TILES = S::TILES, MINE = S::MINE;    /* tiles of the output, those a warp finishes */
+    __shared__ float m_s[W][8 * NT], l_s[W][8 * NT], f_s[W];
+    __shared__ long long scan_s[W + 1];
     __shared__ int find_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t smem0 = (uint32_t)__cvta_generic_to_shared(attn_smem);
     const uint32_t ring = smem0 + S::LUT + warp * S::RING;
-    const uint32_t xchg = smem0 + S::LUT + kAttnWarps * S::RING + 16 * lane;
     const uint32_t lane4 = 4 * lane;                   /* this lane's copy of the table */
 
     if constexpr (F::LUT > 0) {
-        for (int e = warp; e < F::LUT; e += kAttnWarps) *reinterpret_cast<uint32_t*>(attn_smem + 128 * e + lane4) = attn_lut_entry<FMT>(e);
+        for (int e = warp; e < F::LUT; e += W) *reinterpret_cast<uint32_t*>(attn_smem + 128 * e + lane4) = attn_lut_entry<FMT>(e);
     }
     pdl_wait();
 
     /* This CTA's part of the line: sum the sequences' blocks, then find where the part begins. Each
      * item counts kAttnItemCost places more than it has blocks, ahead of its first block. */
     const int items = A.n_kv * A.head_blocks;
-    const int per = (A.n_seqs + 32 * kAttnWarps - 1) / (32 * kAttnWarps);
+    const int per = (A.n_seqs + 32 * W - 1) / (32 * W);
     const int s0 = min(tid * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
     long long mine = 0;
     for (int b = s0; b < s1; b++) mine += attn_places<F::BLOCK>(attn_keys(A, b));
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     __syncthreads();
     long long total = 0, before = upto - mine;
 #pragma unroll
-    for (int w = 0; w < kAttnWarps; w++) {
+    for (int w = 0; w < W; w++) {
         if (w < warp) before += scan_s[w];
         total += scan_s[w];
     }
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
             const int np = attn_places<F::BLOCK>(attn_keys(A, b));
             if (u0 < (at + np) * items) {
                 find_s = b;
-                scan_s[kAttnWarps] = u0 - at * items;
+                scan_s[W] = u0 - at * items;
                 break;
             }
             at += np;
@@ -505,9 +505,9 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     for (int b = part; b < A.n_seqs; b += gridDim.x) {
         if (attn_keys(A, b) > 0) continue;
         uint32_t* o = reinterpret_cast<uint32_t*>(A.out + (size_t)b * A.n_q * HD);
-        for (int i = tid; i < A.n_q * HD / 2; i += 32 * kAttnWarps) o[i] = 0;
+        for (int i = tid; i < A.n_q * HD / 2; i += 32 * W) o[i] = 0;
         if (A.lse != nullptr)
-            for (int i = tid; i < A.n_q; i += 32 * kAttnWarps) A.lse[(size_t)b * A.n_q + i] = -INFINITY;
+            for (int i = tid; i < A.n_q; i += 32 * W) A.lse[(size_t)b * A.n_q + i] = -INFINITY;
         if (A.by_item && tid < items) A.desc[b * items + tid] = make_int2(-1, 0);
     }
     __syncthreads();
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
     AttnAt<F::BLOCK> to, at;                                     /* what is copied next, what is computed next */
     int places = (int)(u1 - u0), skipped = 0;          /* of the line that are left to this CTA */
     if (places > 0) {
-        const long long in = scan_s[kAttnWarps];
+        const long long in = scan_s[W];
         const int b = find_s, np = attn_places<F::BLOCK>(attn_keys(A, b)), item = (int)(in / np);
         const int off = (int)(in - (long long)item * np);
         to.set(A, b, item, max(off - kAttnItemCost, 0));
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
             at = nx;
             continue;
         }
-        /* the item (or the part) ends: join the four warps; warp d finishes tiles d * MINE .. + MINE - 1 */
+        /* the item (or the part) ends: join the warps; warp d finishes tiles d * MINE .. + MINE - 1 */
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -844,86 +844,69 @@ __global__ void __launch_bounds__(32 * kAttnWarps, AttnShape<FMT, HD, NT>::CTAS)
         const bool whole = began && item_done;
         const int slot = 2 * part + (began ? 1 : 0);               /* an item that began here is this CTA's last */
         if (A.by_item && whole && tid == 0) A.desc[at.b * items + at.h] = make_int2(-1, 0);
-        float top[NT][2], sum[NT][2], f[NT][kAttnWarps][2];
+        /* each warp leaves its output in the stage that it has read last, which nothing is copied into before the
+         * next step */
 #pragma unroll
-        for (int round = 0; round < S::ROUNDS; round++) {
-            __syncthreads();                           /* what the exchange held has been read */
-            if (round == 0) {
+        for (int nt = 0; nt < NT; nt++) {
+            if (g == 0) {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-                    if (g == 0) {
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            m_s[warp][8 * nt + 2 * t + c] = m[nt][c];
-                            l_s[warp][8 * nt + 2 * t + c] = l[nt][c];
-                        }
-                    }
-                if (lane == 0) f_s[warp] = vref;
-            }
-#pragma unroll
-            for (int x = 0; x < NT * TILES; x++) {
-                const int d = x / MINE, k = (warp - d - 1) & (kAttnWarps - 1);
-                if ((x % MINE) / S::PER_ROUND != round) continue;
-                if (d != warp) {
-                    const float(&v)[4] = o[x / TILES][x % TILES];
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(xchg + ((d * (kAttnWarps - 1) + k) * S::PER_ROUND + x % S::PER_ROUND) * 512),
-                                 "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
+                for (int c = 0; c < 2; c++) {
+                    m_s[warp][8 * nt + 2 * t + c] = m[nt][c];
+                    l_s[warp][8 * nt + 2 * t + c] = l[nt][c];
                 }
             }
-            __syncthreads();
-            if (round == 0) {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+            for (int j = 0; j < TILES; j++)
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(base + 16 * lane + (nt * TILES + j) * 512),
+                             "f"(o[nt][j][0]), "f"(o[nt][j][1]), "f"(o[nt][j][2]), "f"(o[nt][j][3]) : "memory");
+        }
+        if (lane == 0) f_s[warp] = vref;
+        __syncthreads();
+        {
+            const int nt = warp * MINE / TILES;        /* a warp's tiles are of one column tile */
+            float top[2], sum[2], f[W][2];
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int h = 8 * nt + 2 * t + c;
-                        top[nt][c] = m_s[0][h];
+            for (int c = 0; c < 2; c++) {
+                const int h = 8 * nt + 2 * t + c;
+                top[c] = m_s[0][h];
 #pragma unroll
-                        for (int w = 1; w < kAttnWarps; w++) top[nt][c] = fmaxf(top[nt][c], m_s[w][h]);
-                        sum[nt][c] = 0.0f;
+                for (int w = 1; w < W; w++) top[c] = fmaxf(top[c], m_s[w][h]);
+                sum[c] = 0.0f;
 #pragma unroll
-                        for (int w = 0; w < kAttnWarps; w++) {
-                            f[nt][w][c] = ex2(m_s[w][h] - top[nt][c]);
-                            sum[nt][c] += f[nt][w][c] * l_s[w][h];
-                            f[nt][w][c] *= f_s[w] * (1.0f / attn_alpha<FMT>());
-                        }
-                        if (warp == 0 && g == 0) {
-                            if (!whole) A.part_ml[(size_t)slot * (8 * NT) + h] = make_float2(top[nt][c], sum[nt][c]);
-                            else if (A.lse != nullptr && h < heads) A.lse[head0 + h] = attn_lse(top[nt][c], sum[nt][c]);
-                        }
-                    }
+                for (int w = 0; w < W; w++) {
+                    f[w][c] = ex2(m_s[w][h] - top[c]);
+                    sum[c] += f[w][c] * l_s[w][h];
+                    f[w][c] *= f_s[w] * (1.0f / attn_alpha<FMT>());
+                }
+                if (warp * MINE % TILES == 0 && g == 0) {
+                    if (!whole) A.part_ml[(size_t)slot * (8 * NT) + h] = make_float2(top[c], sum[c]);
+                    else if (A.lse != nullptr && h < heads) A.lse[head0 + h] = attn_lse(top[c], sum[c]);
+                }
             }
+            const uint32_t from = base - warp * S::RING + 16 * lane + warp * MINE * 512;
 #pragma unroll
-            for (int x = 0; x < NT * TILES; x++) {
-                if ((x % MINE) / S::PER_ROUND != round || x / MINE != warp) continue;
-                const int nt = x / TILES, j = x % TILES;
+            for (int k = 0; k < MINE; k++) {
+                const int x = warp * MINE + k, j = x % TILES;
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 0; w < kAttnWarps; w++) { /* in warp order, whoever adds */
+                for (int w = 0; w < W; w++) {          /* in warp order, whoever adds */
                     float v[4];
-                    if (w == warp) {
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(from + w * S::RING + k * 512));
 #pragma unroll
-                        for (int c = 0; c < 4; c++) v[c] = o[nt][j][c];
-                    } else {
-                        const int k = (w - warp - 1) & (kAttnWarps - 1);
-                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                                     : "r"(xchg + ((warp * (kAttnWarps - 1) + k) * S::PER_ROUND + x % S::PER_ROUND) * 512));
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[c] = fmaf(v[c], f[nt][w][c & 1], acc[c]);
+                    for (int c = 0; c < 4; c++) acc[c] = fmaf(v[c], f[w][c & 1], acc[c]);
                 }
                 if (whole) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const int h = 8 * nt + 2 * t + c;
-                        if (h < heads) attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(acc[c], acc[c + 2], sum[nt][c]));
+                        if (h < heads) attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(acc[c], acc[c + 2], sum[c]));
                     }
                 } else {
                     A.part_o[((size_t)slot * (NT * TILES) + x) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 }
             }
         }
+        __syncthreads();                               /* all has been read */
         if (!more) break;
         places -= kAttnItemCost;
         at = nx;
@@ -962,7 +945,7 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
     pdl_wait();
     const int per = A.by_item ? 1 : kAttnJoinParts, mine = blockIdx.x * per + lane;
     int2 d = make_int2(-1, 0);
-    if (lane < per && (A.by_item || mine < kAttnParts)) d = A.desc[mine];
+    if (lane < per && (A.by_item || mine < A.parts)) d = A.desc[mine];
     unsigned todo = __ballot_sync(0xffffffffu, d.x >= 0);
     for (int n = 0; todo != 0; todo &= todo - 1) {
         const int i = __ffs(todo) - 1, which = blockIdx.x * per + i;
@@ -1024,23 +1007,25 @@ static AttnScratch attn_scratch(int group, int head_dim) {
 }
 
 template <int FMT, int HD, int NT>
-static cudaError_t launch_attn(const AttnArgs& A, cudaStream_t s) {
-    constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM;
+static cudaError_t launch_attn(AttnArgs A, cudaStream_t s) {
+    constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM, parts = AttnShape<FMT, HD, NT>::CTAS * kAttnSms;
+    static_assert(parts <= kAttnParts, "the scratch holds kAttnParts parts");
+    A.parts = parts;
     cudaError_t e = cudaFuncSetAttribute((const void*)attn_decode_kernel<FMT, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     /* Even parts want evenly filled SMs. A CTA that is placed while the kernel before still holds some of them
      * starts where there is room, and its part ends late (64 x 4096: 107 us instead of 86, behind a kernel of 888
      * small CTAs), so this is an ordinary launch unless there are few items: then the launch itself is what counts. */
     if (A.by_item) {
-        e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(kAttnParts), dim3(32 * kAttnWarps), (size_t)SMEM, s, A);
+        e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(parts), dim3(32 * AttnFmt<FMT, HD>::W), (size_t)SMEM, s, A);
     } else {
-        attn_decode_kernel<FMT, HD, NT><<<dim3(kAttnParts), dim3(32 * kAttnWarps), (size_t)SMEM, s>>>(A);
+        attn_decode_kernel<FMT, HD, NT><<<dim3(parts), dim3(32 * AttnFmt<FMT, HD>::W), (size_t)SMEM, s>>>(A);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
     constexpr int TILES = NT * (HD / 16);
     if (A.by_item) e = launch_pdl(attn_join_kernel<FMT, HD, NT, 8>, dim3(A.n_seqs * A.n_kv * A.head_blocks, TILES), dim3(256), 0, s, A);
-    else e = launch_pdl(attn_join_kernel<FMT, HD, NT, 4>, dim3((kAttnParts + kAttnJoinParts - 1) / kAttnJoinParts, TILES), dim3(128), 0, s, A);
+    else e = launch_pdl(attn_join_kernel<FMT, HD, NT, 4>, dim3((parts + kAttnJoinParts - 1) / kAttnJoinParts, TILES), dim3(128), 0, s, A);
     if (e == cudaSuccess) g_launches.fetch_add(2, std::memory_order_relaxed);
     return e;
 }
@@ -1075,7 +1060,7 @@ extern "C" int vvbk_attn_decode(const void* q, void* out, float* lse, const void
                         (int2*)base, (float2*)(base + sc.ml), (float4*)(base + sc.o),
                         n_seqs, n_q_heads, n_kv_heads, n_slots, table_stride, len_add,
                         group, (group + 8 * nt - 1) / (8 * nt),
-                        (long long)n_seqs * n_kv_heads * ((group + 8 * nt - 1) / (8 * nt)) <= kAttnFewItems, scale * kLog2e};
+                        0, (long long)n_seqs * n_kv_heads * ((group + 8 * nt - 1) / (8 * nt)) <= kAttnFewItems, scale * kLog2e};
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
     switch (kv_format) {
