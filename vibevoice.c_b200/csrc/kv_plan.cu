@@ -14,12 +14,15 @@
  * it as they are: no second pass and no order that depends on timing.
  *
  * Shape: one CTA, or one cluster of eight for long row lists. Every CTA works
- * out the sums by itself (8 bytes a sequence, from L2) and keeps each
- * sequence's first row and first position in shared memory; CTA 0 writes what
- * is per sequence; the rows are split over the CTAs, each thread four
- * consecutive rows (16-byte stores) after one binary search. Two cluster
- * barriers order the releases before the pages taken, and the tables before the
- * rows that look pages up in them.
+ * out the sums by itself (8 bytes a sequence, from L2) and keeps them in shared
+ * memory, 20 bytes a sequence; from there everything is flat: released pages,
+ * new pages and rows are each split over all threads, which find their sequence
+ * by a binary search in the sums (a loop over its pages by the thread that owns
+ * a sequence took 31 us where this takes XX, at 2000 sequences of up to 256
+ * pages and 131072 rows). One cluster barrier: the released pages are on the
+ * stack, and lens and the stack's height are read, before pages are taken from
+ * it and those are overwritten. Rows do not wait for the tables: a row's page is
+ * either in the table from before or at a known place of the stack.
  */
 #include "vvb_device.cuh"
 #include "vvb_launch.h"
@@ -83,26 +86,26 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-struct PlanSeq {
-    unsigned add, have, released, want;     /* rows, pages held, pages given back, pages asked for */
-    bool full;
-    __device__ __forceinline__ PlanSeq(const PlanArgs& A, int b) {
-        const int n = A.new_tokens[b];
-        const unsigned len = (unsigned)max(A.lens[b], 0);
-        add = (unsigned)max(n, 0);
-        const unsigned cap = (unsigned)A.table_stride << kPlanPageShift;         /* < 2^31 */
-        have = min((len + 63u) >> kPlanPageShift, (unsigned)A.table_stride);
-        released = n < 0 ? have : 0u;
-        full = n >= 0 && (len > cap || add > cap - len);
-        want = (n < 0 || full) ? 0u : ((len + add + 63u) >> kPlanPageShift) - have;
+/* Largest i in [0, n) with a[i] <= x, for ascending a and a[0] <= x < a[n]: among equal entries the last, so that
+ * entry's part is not empty. */
+__device__ __forceinline__ int plan_find(const unsigned* a, int n, unsigned x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= x) lo = mid; else hi = mid;
     }
-};
+    return lo;
+}
 
 template <bool CLUSTER>
 __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant__ PlanArgs A) {
-    extern __shared__ int plan_smem[];
-    int* const start_s = plan_smem;                     /* [n_seqs + 1] first row of each sequence */
-    int* const base_s = plan_smem + A.n_seqs + 1;       /* [n_seqs] its first new position, -1 when refused or released */
+    extern __shared__ unsigned plan_smem[];
+    const int n = A.n_seqs;
+    unsigned* const start_s = plan_smem;                       /* [n + 1] first row of each sequence */
+    unsigned* const push_s = plan_smem + n + 1;                /* [n + 1] its first released page */
+    unsigned* const take_s = plan_smem + 2 * (n + 1);          /* [n + 1] its first new page */
+    int* const new_s = reinterpret_cast<int*>(plan_smem + 3 * (n + 1));      /* [n] new tokens */
+    int* const base_s = new_s + n;                             /* [n] cached positions; then -1 when refused or released */
     __shared__ unsigned ws[64];
     __shared__ unsigned taken_s;
     const int t = threadIdx.x, nt = blockDim.x;
@@ -111,106 +114,106 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
     pdl_wait();
     pdl_trigger();
 
-    const int per = (A.n_seqs + nt - 1) / nt;
-    const int b0 = min(t * per, A.n_seqs), b1 = min(b0 + per, A.n_seqs);
+    const unsigned cap = (unsigned)A.table_stride << kPlanPageShift;         /* < 2^31 */
+    auto pages_of = [&](int len) { return min(((unsigned)len + 63u) >> kPlanPageShift, (unsigned)A.table_stride); };
+    auto full = [&](int add, int len) { return add >= 0 && ((unsigned)len > cap || (unsigned)add > cap - (unsigned)len); };
+    const unsigned held = (unsigned)min(max(__ldg(A.free_count), 0), A.n_pages);
+    const int per = (n + nt - 1) / nt;
+    const int b0 = min(t * per, n), b1 = min(b0 + per, n);
     /* rows and released pages */
     unsigned rows = 0, rel = 0;
     for (int b = b0; b < b1; b++) {
-        const PlanSeq s(A, b);
-        rows = sat_add(rows, s.add);
-        rel = sat_add(rel, s.released);
+        const int add = __ldg(A.new_tokens + b), len = max(__ldg(A.lens + b), 0);
+        new_s[b] = add;
+        base_s[b] = len;
+        rows = sat_add(rows, (unsigned)max(add, 0));
+        rel = sat_add(rel, add < 0 ? pages_of(len) : 0u);
     }
-    unsigned row0, rel0, rows_total, rel_total;
-    block_scan2(rows, rel, ws, row0, rel0, rows_total, rel_total);
-    /* pages asked for, by the sequences whose rows fit */
-    unsigned want = 0, row = row0;
+    unsigned row, push, rows_total, rel_total;
+    block_scan2(rows, rel, ws, row, push, rows_total, rel_total);
+    /* pages asked for, by the sequences that have a table and rows for them */
+    unsigned want = 0;
     for (int b = b0; b < b1; b++) {
-        const PlanSeq s(A, b);
-        row = sat_add(row, s.add);
-        if (row <= (unsigned)A.max_rows) want = sat_add(want, s.want);   /* (no rows: nothing wanted either) */
+        const int add = new_s[b], len = base_s[b];
+        start_s[b] = row;
+        push_s[b] = push;
+        row = sat_add(row, (unsigned)max(add, 0));
+        push = sat_add(push, add < 0 ? pages_of(len) : 0u);
+        if (add > 0 && row <= (unsigned)A.max_rows && !full(add, len))
+            want = sat_add(want, (((unsigned)len + (unsigned)add + 63u) >> kPlanPageShift) - pages_of(len));
     }
-    unsigned want0, unused0, want_total, unused1;
-    block_scan2(want, 0u, ws, want0, unused0, want_total, unused1);
-
-    const unsigned held = (unsigned)min(max(*A.free_count, 0), A.n_pages);
+    unsigned upto, unused0, want_total, unused1;
+    block_scan2(want, 0u, ws, upto, unused0, want_total, unused1);
     const unsigned avail = min(sat_add(held, rel_total), (unsigned)A.n_pages);
-    /* what is per sequence: kept in shared memory by every CTA, written by the first */
-    unsigned push = rel0, upto = want0;
-    row = row0;
+    row = b0 < b1 ? start_s[b0] : 0u;
     for (int b = b0; b < b1; b++) {
-        const PlanSeq s(A, b);
-        const unsigned end = sat_add(row, s.add);
-        const bool no_rows = s.add > 0 && !s.full && end > (unsigned)A.max_rows;
-        const unsigned ask = no_rows ? 0u : s.want;
-        const unsigned total = sat_add(upto, ask);
-        const bool no_pages = ask > 0 && total > avail;
-        const bool ends = A.new_tokens[b] < 0;
-        const bool ok = !(s.full || no_rows || no_pages || ends);
-        const int len = max(A.lens[b], 0);
-        start_s[b] = (int)row;
+        const int add = new_s[b], len = base_s[b];
+        row = sat_add(row, (unsigned)max(add, 0));
+        const bool no_table = full(add, len), no_rows = add > 0 && !no_table && row > (unsigned)A.max_rows;
+        const unsigned ask = add > 0 && !no_table && !no_rows ? (((unsigned)len + (unsigned)add + 63u) >> kPlanPageShift) - pages_of(len) : 0u;
+        take_s[b] = upto;
+        upto = sat_add(upto, ask);
+        const bool no_pages = ask > 0 && upto > avail;
+        const bool ok = !(no_table || no_rows || no_pages || add < 0);
+        if (ok && ask > 0) atomicMax(&taken_s, upto);
         base_s[b] = ok ? len : -1;
-        if (ok && ask > 0) atomicMax(&taken_s, total);
         if (rank == 0) {
-            A.row_start[b] = (int)row;
-            if (A.status != nullptr) A.status[b] = s.full ? 2 : no_rows ? 3 : no_pages ? 1 : 0;
-            const int* mine = A.block_table + (size_t)b * A.table_stride;
-            for (unsigned k = 0; k < s.released; k++) {
-                const unsigned at = held + push + k;
-                if (at < (unsigned)A.n_pages) A.free_pages[at] = mine[k];
-            }
+            A.row_start[b] = (int)start_s[b];
+            if (A.status != nullptr) A.status[b] = no_table ? 2 : no_rows ? 3 : no_pages ? 1 : 0;
         }
-        push = sat_add(push, s.released);
-        upto = total;
-        row = end;
     }
-    if (t == 0) start_s[A.n_seqs] = (int)rows_total;
-    if (rank == 0 && t == 0) A.row_start[A.n_seqs] = (int)rows_total;
+    if (t == 0) {
+        start_s[n] = rows_total;
+        push_s[n] = rel_total;
+        take_s[n] = want_total;
+        if (rank == 0) A.row_start[n] = (int)rows_total;
+    }
     __syncthreads();
-    if (CLUSTER) cluster_barrier();      /* all CTAs have read lens; the released pages are on the stack */
+    const unsigned taken = taken_s;                            /* pages 0 .. taken - 1 of the call are given out */
+    const int first = rank * nt + t, step = ranks * nt;
+
+    /* released pages onto the stack */
+    for (unsigned i = first; i < rel_total && held + i < (unsigned)A.n_pages; i += step) {
+        const int b = plan_find(push_s, n, i);
+        A.free_pages[held + i] = A.block_table[(size_t)b * A.table_stride + (i - push_s[b])];
+    }
+    __syncthreads();
+    if (CLUSTER) cluster_barrier();      /* all CTAs have read lens and the height; the released pages are on the stack */
 
     if (rank == 0) {
-        upto = want0;
-        for (int b = b0; b < b1; b++) {
-            const PlanSeq s(A, b);                       /* this thread has not yet overwritten these */
-            const unsigned ask = (!s.full && sat_add((unsigned)start_s[b], s.add) > (unsigned)A.max_rows) ? 0u : s.want;
-            if (base_s[b] >= 0) {
-                int* mine = A.block_table + (size_t)b * A.table_stride + s.have;
-                for (unsigned k = 0; k < ask; k++) mine[k] = __ldcg(A.free_pages + (avail - 1u - upto - k));
-            }
-            upto = sat_add(upto, ask);
-            A.lens_out[b] = A.new_tokens[b] < 0 ? 0 : base_s[b] >= 0 ? base_s[b] + (int)s.add : A.lens[b];
+        for (int b = t; b < n; b += nt) {
+            const int add = new_s[b];
+            if (add < 0) A.lens_out[b] = 0;
+            else if (base_s[b] >= 0) A.lens_out[b] = base_s[b] + add;
+            else if (A.lens_out != A.lens) A.lens_out[b] = A.lens[b];
         }
-        if (t == 0) *A.free_count_out = (int)(avail - taken_s);
+        if (t == 0) *A.free_count_out = (int)(avail - taken);
     }
-    __syncthreads();
-    if (CLUSTER) cluster_barrier();      /* the tables are written */
-
+    /* new pages into the tables, page j from the j-th place below the stack's top */
+    for (unsigned j = first; j < taken; j += step) {
+        const int b = plan_find(take_s, n, j);
+        if (base_s[b] >= 0) A.block_table[(size_t)b * A.table_stride + pages_of(base_s[b]) + (j - take_s[b])] = __ldcg(A.free_pages + (avail - 1u - j));
+    }
     /* rows: four consecutive ones a thread */
     const bool vec = ((reinterpret_cast<uintptr_t>(A.slot_map) | reinterpret_cast<uintptr_t>(A.positions)) & 15u) == 0;
-    for (long long r0 = 4ll * (rank * nt + t); r0 < A.max_rows; r0 += 4ll * ranks * nt) {
+    for (long long r0 = 4ll * first; r0 < A.max_rows; r0 += 4ll * step) {
         int slot[4], pos[4];
-        int b = 0;
-        if (r0 < (long long)rows_total) {               /* the last sequence that starts at or before r0 and is not empty there */
-            int lo = 0, hi = A.n_seqs;                   /* start_s[lo] <= r0 < start_s[hi] */
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start_s[mid] <= (int)r0) lo = mid; else hi = mid;
-            }
-            b = lo;
-        }
+        int b = r0 < (long long)rows_total ? plan_find(start_s, n, (unsigned)r0) : 0;
         int page_of = -1, page = 0, seen = -1;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const long long r = r0 + j;
             slot[j] = pos[j] = -1;
             if (r >= A.max_rows || r >= (long long)rows_total) continue;
-            while (start_s[b + 1] <= (int)r) b++;
-            const int first = base_s[b];
-            if (first < 0) continue;
-            const int p = first + (int)r - start_s[b];
+            while (start_s[b + 1] <= (unsigned)r) b++;
+            const int from = base_s[b];
+            if (from < 0) continue;
+            const int p = from + (int)((unsigned)r - start_s[b]);
             const int blk = p >> kPlanPageShift;
             if (blk != page_of || b != seen) {
-                page = __ldcg(A.block_table + (size_t)b * A.table_stride + blk);
+                const int fresh = blk - (int)pages_of(from);
+                page = fresh < 0 ? __ldcg(A.block_table + (size_t)b * A.table_stride + blk)
+                                 : __ldcg(A.free_pages + (avail - 1u - take_s[b] - (unsigned)fresh));
                 page_of = blk;
                 seen = b;
             }
@@ -239,7 +242,7 @@ extern "C" int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_ou
     const PlanArgs A = {new_tokens, lens, lens_out, block_table, free_pages, free_count, free_count_out, row_start,
                         slot_map, positions, status, n_seqs, table_stride, n_pages, max_rows};
     const bool cluster = max_rows > 4096;
-    const size_t smem = (2 * (size_t)n_seqs + 1) * sizeof(int);       /* n_seqs <= 8192: 64 KB */
+    const size_t smem = (5 * (size_t)n_seqs + 3) * sizeof(int);       /* n_seqs <= 8192: 160 KB */
     void (*kernel)(const PlanArgs) = cluster ? kv_plan_kernel<true> : kv_plan_kernel<false>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -247,7 +250,9 @@ extern "C" int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_ou
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cluster ? kPlanCluster : 1);
-    cfg.blockDim = dim3(1024);
+    /* few rows of few sequences: fewer threads, whose barriers are quicker */
+    const int threads = max_rows / 4 > n_seqs ? max_rows / 4 : n_seqs;
+    cfg.blockDim = dim3(cluster || threads > 512 ? 1024u : threads > 128 ? 512u : 128u);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute at[2];
