@@ -13,12 +13,12 @@
  * passes the stack's height is refused, which leaves the sums of those before
  * it as they are: no second pass and no order that depends on timing.
  *
- * Shape: one CTA, or one cluster of eight for long row lists. Every CTA works
+ * Shape: one CTA, or one cluster of 8 or 16 for long row lists. Every CTA works
  * out the sums by itself (8 bytes a sequence, from L2) and keeps them in shared
  * memory, 20 bytes a sequence; from there everything is flat: released pages,
  * new pages and rows are each split over all threads, which find their sequence
  * by a binary search in the sums (a loop over its pages by the thread that owns
- * a sequence took 31 us where this takes XX, at 2000 sequences of up to 256
+ * a sequence took 31 us where this takes 11, at 2000 sequences of up to 256
  * pages and 131072 rows). One cluster barrier: the released pages are on the
  * stack, and lens and the stack's height are read, before pages are taken from
  * it and those are overwritten. Rows do not wait for the tables: a row's page is
@@ -34,7 +34,6 @@ namespace vvb {
 extern std::atomic<uint64_t> g_launches;
 
 constexpr int kPlanPageShift = 6;
-constexpr int kPlanCluster = 8;
 
 struct PlanArgs {
     const int* new_tokens;
@@ -194,39 +193,41 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
         const int b = plan_find(take_s, n, j);
         if (base_s[b] >= 0) A.block_table[(size_t)b * A.table_stride + pages_of(base_s[b]) + (j - take_s[b])] = __ldcg(A.free_pages + (avail - 1u - j));
     }
-    /* rows: four consecutive ones a thread */
+    /* rows: four consecutive ones a thread, each with a page look-up of its own, all in flight at once: a look-up
+     * only where a page or a sequence begins costs its latency once a row, since some lane of a warp is always there */
+    constexpr int kRun = 4;
     const bool vec = ((reinterpret_cast<uintptr_t>(A.slot_map) | reinterpret_cast<uintptr_t>(A.positions)) & 15u) == 0;
-    for (long long r0 = 4ll * first; r0 < A.max_rows; r0 += 4ll * step) {
-        int slot[4], pos[4];
-        int b = r0 < (long long)rows_total ? plan_find(start_s, n, (unsigned)r0) : 0;
-        int page_of = -1, page = 0, seen = -1;
+    const unsigned max_rows = (unsigned)A.max_rows;
+    for (unsigned long long run0 = (unsigned long long)kRun * first; run0 < max_rows; run0 += (unsigned long long)kRun * step) {
+        const unsigned r0 = (unsigned)run0;
+        int b = r0 < rows_total ? plan_find(start_s, n, r0) : 0;
+        int slot[kRun], pos[kRun];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const long long r = r0 + j;
+        for (int j = 0; j < kRun; j++) {
+            const unsigned r = r0 + j;
             slot[j] = pos[j] = -1;
-            if (r >= A.max_rows || r >= (long long)rows_total) continue;
-            while (start_s[b + 1] <= (unsigned)r) b++;
+            if (r >= rows_total || r >= max_rows) continue;
+            while (start_s[b + 1] <= r) b++;
             const int from = base_s[b];
             if (from < 0) continue;
-            const int p = from + (int)((unsigned)r - start_s[b]);
-            const int blk = p >> kPlanPageShift;
-            if (blk != page_of || b != seen) {
-                const int fresh = blk - (int)pages_of(from);
-                page = fresh < 0 ? __ldcg(A.block_table + (size_t)b * A.table_stride + blk)
-                                 : __ldcg(A.free_pages + (avail - 1u - take_s[b] - (unsigned)fresh));
-                page_of = blk;
-                seen = b;
-            }
-            pos[j] = p;
-            slot[j] = (page << kPlanPageShift) + (p & 63);
+            const unsigned p = (unsigned)from + (r - start_s[b]), blk = p >> kPlanPageShift, had = pages_of(from);
+            pos[j] = (int)p;
+            slot[j] = __ldcg(blk < had ? A.block_table + (size_t)b * A.table_stride + blk : A.free_pages + (avail - 1u - take_s[b] - (blk - had)));
         }
-        if (vec && r0 + 4 <= A.max_rows) {
-            *reinterpret_cast<int4*>(A.slot_map + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-            *reinterpret_cast<int4*>(A.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-        } else {
-            for (int j = 0; j < 4 && r0 + j < A.max_rows; j++) {
-                A.slot_map[r0 + j] = slot[j];
-                A.positions[r0 + j] = pos[j];
+#pragma unroll
+        for (int j = 0; j < kRun; j++)
+            if (pos[j] >= 0) slot[j] = (int)(((unsigned)slot[j] << kPlanPageShift) + ((unsigned)pos[j] & 63u));
+#pragma unroll
+        for (int j = 0; j < kRun; j += 4) {
+            if (vec && r0 + j + 4 <= max_rows) {
+                *reinterpret_cast<int4*>(A.slot_map + r0 + j) = make_int4(slot[j], slot[j + 1], slot[j + 2], slot[j + 3]);
+                *reinterpret_cast<int4*>(A.positions + r0 + j) = make_int4(pos[j], pos[j + 1], pos[j + 2], pos[j + 3]);
+            } else {
+                for (int k = j; k < j + 4; k++)
+                    if (r0 + k < max_rows) {
+                        A.slot_map[r0 + k] = slot[k];
+                        A.positions[r0 + k] = pos[k];
+                    }
             }
         }
     }
@@ -241,15 +242,22 @@ extern "C" int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_ou
                             int* status, int n_seqs, int table_stride, int n_pages, int max_rows, void* stream) {
     const PlanArgs A = {new_tokens, lens, lens_out, block_table, free_pages, free_count, free_count_out, row_start,
                         slot_map, positions, status, n_seqs, table_stride, n_pages, max_rows};
-    const bool cluster = max_rows > 4096;
+    /* Rows are what takes time beyond the first few thousand, 1024 threads a CTA; 16 CTAs (the most a cluster can have,
+     * by opt-in) from where that shows: 131072 rows of 2000 sequences 14.6 us with 8, 11.1 with 16. */
+    const int ctas = max_rows > 32768 ? 16 : max_rows > 4096 ? 8 : 1;
+    const bool cluster = ctas > 1;
     const size_t smem = (5 * (size_t)n_seqs + 3) * sizeof(int);       /* n_seqs <= 8192: 160 KB */
     void (*kernel)(const PlanArgs) = cluster ? kv_plan_kernel<true> : kv_plan_kernel<false>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)e;
     }
+    if (ctas > 8) {
+        const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return (int)e;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster ? kPlanCluster : 1);
+    cfg.gridDim = dim3(ctas);
     /* few rows of few sequences: fewer threads, whose barriers are quicker */
     const int threads = max_rows / 4 > n_seqs ? max_rows / 4 : n_seqs;
     cfg.blockDim = dim3(cluster || threads > 512 ? 1024u : threads > 128 ? 512u : 128u);
@@ -259,7 +267,7 @@ extern "C" int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_ou
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = kPlanCluster;
+    at[1].val.clusterDim.x = ctas;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster ? 2 : 1;
