@@ -48,8 +48,13 @@
  * position positions[r], and a row whose slot lies outside the cache (-1: the
  * padding of a batch of fixed capacity, a refused sequence) is left alone
  * altogether, Q included. For every format; an instantiation carries no trace of
- * the other mappings. The slot of a row is loaded beside its data and tested at
- * the store, so that it does not stand before the loads.
+ * the other mappings. Slots and positions are read once a CTA, beside the first
+ * data and not between the data and its store: by a lane for each of a V CTA's 32
+ * rows, through shared memory for a tile's (read by each thread for itself they
+ * cost the FP8 append of 2500 rows 12.2 us instead of 11.2, in spilled registers).
+ * A tile's cos and sin wait for its positions, an L2 latency that nothing of the
+ * tile hides: 14449 rows in FP16 45.6 us, 41.9 with one sequence's page table.
+ * (An L2 prefetch of the positions 512, 2048 or 8192 rows ahead changed nothing.)
  */
 #include "fp8_kv.cuh"
 #include "rope.cuh"
@@ -143,6 +148,11 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
         if (row0v >= a.rows) return;
         const int items = min(kVRowsPerCta, a.rows - row0v) * cols_v;
         const int cache_first_v = (a.d_position != nullptr) ? *a.d_position : A.cache_offset;
+        int slot_v = -1;                                       /* kAddrSlots: of row row0v + lane */
+        if constexpr (ADDR == kAddrSlots) {
+            static_assert(kVRowsPerCta == 32, "a lane holds a row's slot");
+            if (row0v + (t & 31) < a.rows) slot_v = (int)dest_row<ADDR>(A, 0, row0v + (t & 31));
+        }
         if constexpr (kv_is_tq(FMT)) {
             /* eight lanes to a head vector (tq_store16): a warp takes four consecutive vectors a
              * step, each lane two 16-byte pieces of its vector, and has two steps' loads in flight */
@@ -177,9 +187,11 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
                     const int idx = base + j * 4 * kWarps + (lane >> 3);
                     bool live = idx < nvecs;
                     long long row = 0;
-                    if (live) {
+                    if constexpr (ADDR == kAddrSlots) {
+                        row = __shfl_sync(0xffffffffu, slot_v, rl & 31);
+                        if (row < 0) { live = false; row = 0; }
+                    } else if (live) {
                         row = dest_row<ADDR>(A, cache_first_v, row0v + rl);
-                        if (ADDR == kAddrSlots && row < 0) { live = false; row = 0; }
                     }
                     if (A.v_bias && live) {
                         x[j][0] = add_bias_vec(x[j][0], __ldg(A.v_bias + h * 16 + 2 * sub));
@@ -203,7 +215,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             return;
         }
         constexpr int kVUnroll = 4;
-        for (int base = t; base < items; base += kRopeThreads * kVUnroll) {
+        for (int base = t; (ADDR == kAddrSlots ? base - (t & 31) : base) < items; base += kRopeThreads * kVUnroll) {
             vec16 x[kVUnroll];
 #pragma unroll
             for (int j = 0; j < kVUnroll; j++) {
@@ -213,11 +225,16 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
 #pragma unroll
             for (int j = 0; j < kVUnroll; j++) {
                 const int it = base + j * kRopeThreads;
-                if (it >= items) continue;
+                if (ADDR != kAddrSlots && it >= items) continue;
                 const int rl = it / cols_v;
                 const int cv = it - rl * cols_v;
-                const long long row = dest_row<ADDR>(A, cache_first_v, row0v + rl);
-                if (ADDR == kAddrSlots && row < 0) continue;
+                long long row;
+                if constexpr (ADDR == kAddrSlots) {            /* the whole warp is here */
+                    row = __shfl_sync(0xffffffffu, slot_v, rl & 31);
+                    if (it >= items || row < 0) continue;
+                } else {
+                    row = dest_row<ADDR>(A, cache_first_v, row0v + rl);
+                }
                 if (A.v_bias) x[j] = add_bias_vec(x[j], __ldg(A.v_bias + cv));
                 const size_t at = (size_t)row * cols_v + cv;
                 if constexpr (FMT == KV_RAW) st_stream(A.v_cache + at, x[j]);
@@ -286,10 +303,18 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
         if (A.k_bias) bias = A.k_bias + off;
     }
 
+    /* kAddrSlots: slots and positions of the tile's rows (at most kRopeTableEntries / 8 of them) */
+    __shared__ int slot_s[ADDR == kAddrSlots ? kRopeTableEntries / 8 : 1], pos_s[ADDR == kAddrSlots ? kRopeTableEntries / 8 : 1];
+    int slot_t = -1, pos_t = 0;
+    if constexpr (ADDR == kAddrSlots) {
+        if (t < nrows) {
+            slot_t = (int)dest_row<ADDR>(A, 0, row0 + t);
+            pos_t = __ldg(A.positions + row0 + t);
+        }
+    }
     /* Phase A: loads in flight. */
     vec16 lo[kRopeMaxRowsPerThread], hi[kRopeMaxRowsPerThread];
     bool live[kRopeMaxRowsPerThread];
-    int slot_of[kRopeMaxRowsPerThread];                    /* kAddrSlots */
     vec16 blo = make_uint4(0, 0, 0, 0), bhi = make_uint4(0, 0, 0, 0);
     if (col_ok && bias != nullptr) {
         blo = __ldg(bias);
@@ -303,16 +328,22 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             const vec16* p = src + (size_t)(row0 + rl) * stride;
             lo[m] = ld_stream(p);
             hi[m] = ld_stream(p + a.hvn);
-            if constexpr (ADDR == kAddrSlots) slot_of[m] = (int)dest_row<ADDR>(A, 0, row0 + rl);
         }
     }
 
+    if constexpr (ADDR == kAddrSlots) {
+        if (t < nrows) {
+            slot_s[t] = slot_t;
+            pos_s[t] = pos_t;
+        }
+        __syncthreads();
+    }
     /* Phase B: cos/sin of the CTA's rows. */
     const int pos0 = pos_first + row0;
     for (int e = t; e < nrows * a.half; e += kRopeThreads) {
         const int rl = e / a.half;
         const int i = e - rl * a.half;
-        const int pos = (ADDR == kAddrSlots) ? __ldg(A.positions + row0 + rl) : pos0 + rl;
+        const int pos = (ADDR == kAddrSlots) ? pos_s[ADDR == kAddrSlots ? rl : 0] : pos0 + rl;
         const float ang = __fmul_rn((float)pos, a.inv_freq[i]);
         sincos_f64(ang, &sin_s[e], &cos_s[e]);
     }
@@ -322,8 +353,9 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
 #pragma unroll
     for (int m = 0; m < kRopeMaxRowsPerThread; m++) {
         if (!live[m]) continue;
-        if (ADDR == kAddrSlots && slot_of[m] < 0) continue;
         const int rl = slot + m * a.row_slots;
+        const int slot_r = (ADDR == kAddrSlots) ? slot_s[ADDR == kAddrSlots ? rl : 0] : 0;
+        if (ADDR == kAddrSlots && slot_r < 0) continue;
         vec16 xlo = lo[m], xhi = hi[m];
         if (bias != nullptr) {
             xlo = add_bias_vec(xlo, blo);
@@ -354,7 +386,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             if constexpr (FMT != KV_RAW && !kv_is_tq(FMT)) {
                 /* one byte per element: vector i of the row is 8 bytes at uint2 index i */
                 uint2* d8 = reinterpret_cast<uint2*>(A.k_cache) +
-                            ((size_t)(ADDR == kAddrSlots ? slot_of[m] : dest_row<ADDR>(A, dst_row_first, row0 + rl)) * stride +
+                            ((size_t)(ADDR == kAddrSlots ? slot_r : dest_row<ADDR>(A, dst_row_first, row0 + rl)) * stride +
                              (size_t)(dst - A.k_cache));
                 const bool sub = A.k_ref != nullptr;
                 __stcs(d8, fp8_encode8<FMT>(xlo, sub ? &rlo : nullptr));
@@ -363,7 +395,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             /* (a TurboQuant launch always stages: the launcher plans the tile to fit) */
         } else {
             const size_t drow = !to_cache ? (size_t)(row0 + rl)
-                                : (size_t)(ADDR == kAddrSlots ? slot_of[m] : dest_row<ADDR>(A, dst_row_first, row0 + rl));
+                                : (size_t)(ADDR == kAddrSlots ? slot_r : dest_row<ADDR>(A, dst_row_first, row0 + rl));
             vec16* d = dst + drow * stride;
             st_stream(d, xlo);
             st_stream(d + a.hvn, xhi);
@@ -400,7 +432,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             for (int base = 4 * warp; base < total; base += 4 * kWarps) {          /* warp-uniform */
                 bool live = base + (lane >> 3) < total;
                 const int rs = live ? rl : 0, hs = live ? hk : 0;
-                long long row = dest_row<ADDR>(A, cache_first, row0 + rs);
+                long long row = (ADDR == kAddrSlots) ? slot_s[ADDR == kAddrSlots ? rs : 0] : dest_row<ADDR>(A, cache_first, row0 + rs);
                 if (ADDR == kAddrSlots && row < 0) { live = false; row = 0; }
                 const vec16* src16 = &k_stage[(rs * 2 + half_sel) * kcols + hs * a.hvn + vsel];
                 const vec16 x0 = src16[0], x1 = src16[1];
@@ -443,7 +475,7 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
             const int ck = first_k_col + kc;
             const int hd = ck / a.hvn;
             const size_t off = (size_t)(hd - a.n_q) * vph + (size_t)(ck - hd * a.hvn) + ((rh & 1) ? (size_t)a.hvn : 0);
-            const long long row = dest_row<ADDR>(A, cache_first, row0 + rl);
+            const long long row = (ADDR == kAddrSlots) ? slot_s[ADDR == kAddrSlots ? rl : 0] : dest_row<ADDR>(A, cache_first, row0 + rl);
             if (ADDR == kAddrSlots && row < 0) continue;
             uint2* d8 = reinterpret_cast<uint2*>(A.k_cache) + ((size_t)row * stride_k + off);
             const vec16 x = k_stage[idx];
