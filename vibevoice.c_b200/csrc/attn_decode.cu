@@ -86,7 +86,7 @@ struct AttnArgs {
     int n_seqs, n_q, n_kv, n_slots, table_stride, len_add;
     int group, head_blocks;    /* query heads to a cache head, items a cache head is cut into */
     int parts;                 /* CTAs of the launch */
-    int by_item;
+    int by_item, whole_items;
     float scale2;              /* scale * log2(e) */
 };
 
@@ -445,64 +445,89 @@ template <int BLOCK> struct AttnAt {
     }
 };
 
-template <int FMT, int HD, int NT>
+/* The line of `total` places cut into `parts` equal parts: place where part p begins, floor(total p / parts). */
+struct AttnCut {
+    long long each;
+    unsigned rest, parts;
+    __device__ __forceinline__ AttnCut(long long total, int n) : parts((unsigned)n) {
+        each = total <= 0xffffffffll ? (long long)((unsigned)total / (unsigned)n) : total / n;
+        rest = (unsigned)(total - each * n);
+    }
+    __device__ __forceinline__ long long at(unsigned p) const { return each * p + rest * p / parts; }
+};
+
+template <int FMT, int HD, int NT, bool SOLO>
 __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, NT>::CTAS) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
     using F = AttnFmt<FMT, HD>;
     using S = AttnShape<FMT, HD, NT>;
     constexpr bool TQ = kv_is_tq(FMT);
     constexpr int W = F::W, TILES = S::TILES, MINE = S::MINE;    /* tiles of the output, those a warp finishes */
+    constexpr int BLOCK = SOLO ? F::KEYS : F::BLOCK;   /* a warp alone takes a block by itself */
     __shared__ float m_s[W][8 * NT], l_s[W][8 * NT], f_s[W];
-    __shared__ long long scan_s[W + 1];
-    __shared__ int find_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int warp_key = SOLO ? 0 : F::KEYS * warp;    /* of the block: the warp's first */
     const uint32_t smem0 = (uint32_t)__cvta_generic_to_shared(attn_smem);
     const uint32_t ring = smem0 + S::LUT + warp * S::RING;
     const uint32_t lane4 = 4 * lane;                   /* this lane's copy of the table */
 
     if constexpr (F::LUT > 0) {
         for (int e = warp; e < F::LUT; e += W) *reinterpret_cast<uint32_t*>(attn_smem + 128 * e + lane4) = attn_lut_entry<FMT>(e);
+        __syncthreads();
     }
     pdl_wait();
 
-    /* This CTA's part of the line: sum the sequences' blocks, then find where the part begins. Each
-     * item counts kAttnItemCost places more than it has blocks, ahead of its first block. */
+    /* This CTA's (SOLO: warp's) part of the line: sum the sequences' blocks, then find where the part begins. Each
+     * item counts kAttnItemCost places more than it has blocks, ahead of its first block. Every warp does it for
+     * itself, a lane for every 32nd of the sequences. */
     const int items = A.n_kv * A.head_blocks;
-    const int per = (A.n_seqs + 32 * W - 1) / (32 * W);
-    const int s0 = min(tid * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
+    const bool whole_items = SOLO || A.whole_items;    /* an item belongs to the part in which it begins */
+    const int per = (A.n_seqs + 31) / 32;
+    const int s0 = min(lane * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
     long long mine = 0;
-    for (int b = s0; b < s1; b++) mine += attn_places<F::BLOCK>(attn_keys(A, b));
+#pragma unroll 4
+    for (int b = s0; b < s1; b++) mine += attn_places<BLOCK>(attn_keys(A, b));
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
     }
-    if (lane == 31) scan_s[warp] = upto;
-    __syncthreads();
-    long long total = 0, before = upto - mine;
-#pragma unroll
-    for (int w = 0; w < W; w++) {
-        if (w < warp) before += scan_s[w];
-        total += scan_s[w];
-    }
-    total *= items;
-    const int parts = (int)min((long long)gridDim.x, total / (1 + kAttnItemCost));
-    const int part = blockIdx.x;
-    const long long u0 = part < parts ? total * part / parts : 0, u1 = part < parts ? total * (part + 1) / parts : 0;
-    if (u0 < u1 && mine > 0 && u0 >= before * items && u0 < (before + mine) * items) {
-        long long at = before;                         /* one thread finds itself here */
-        for (int b = s0; b < s1; b++) {
-            const int np = attn_places<F::BLOCK>(attn_keys(A, b));
-            if (u0 < (at + np) * items) {
-                find_s = b;
-                scan_s[W] = u0 - at * items;
-                break;
+    const long long total = __shfl_sync(0xffffffffu, upto, 31) * items, before = (upto - mine) * items;
+    const int part = SOLO ? blockIdx.x * W + warp : blockIdx.x;
+    const int parts = (int)max(min((long long)(SOLO ? gridDim.x * W : gridDim.x), total / (1 + kAttnItemCost)), 1ll);
+    const AttnCut cut(total, parts);
+    const long long u0 = part < parts ? cut.at(part) : total, u1 = part < parts ? cut.at(part + 1) : total;
+
+    AttnAt<BLOCK> to, at;                              /* what is copied next, what is computed next */
+    int places = (int)(u1 - u0), skipped = 0;          /* of the line that are left to this part */
+    if (places > 0) {
+        const int who = __ffs(__ballot_sync(0xffffffffu, u0 >= before && u0 < before + mine * items)) - 1;
+        int b = 0;
+        long long in = 0;                              /* place in sequence b's stretch of the line */
+        if (lane == who) {
+            in = u0 - before;
+            for (b = s0; b < s1; b++) {
+                const long long stretch = (long long)attn_places<BLOCK>(attn_keys(A, b)) * items;
+                if (in < stretch) break;
+                in -= stretch;
             }
-            at += np;
         }
+        b = __shfl_sync(0xffffffffu, b, who);
+        in = __shfl_sync(0xffffffffu, in, who);
+        const int np = attn_places<BLOCK>(attn_keys(A, b));
+        const int item = in <= 0xffffffffll ? (int)((unsigned)in / (unsigned)np) : (int)(in / np);
+        const int off = (int)(in - (long long)item * np);
+        to.set(A, b, item, max(off - kAttnItemCost, 0));
+        skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
+        if (whole_items && off > 0) {                  /* begun in an earlier part */
+            skipped = np - off + kAttnItemCost;
+            if (places > np - off) to.next_item(A, items);
+        }
+        places -= skipped;
+        if (whole_items) places = places + kAttnItemCost > 0 ? max(places, 1) : 0;
     }
     /* rows without keys */
-    for (int b = part; b < A.n_seqs; b += gridDim.x) {
+    for (int b = blockIdx.x; b < A.n_seqs; b += gridDim.x) {
         if (attn_keys(A, b) > 0) continue;
         uint32_t* o = reinterpret_cast<uint32_t*>(A.out + (size_t)b * A.n_q * HD);
         for (int i = tid; i < A.n_q * HD / 2; i += 32 * W) o[i] = 0;
@@ -510,37 +535,12 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
             for (int i = tid; i < A.n_q; i += 32 * W) A.lse[(size_t)b * A.n_q + i] = -INFINITY;
         if (A.by_item && tid < items) A.desc[b * items + tid] = make_int2(-1, 0);
     }
-    __syncthreads();
-
-    AttnAt<F::BLOCK> to, at;                                     /* what is copied next, what is computed next */
-    int places = (int)(u1 - u0), skipped = 0;          /* of the line that are left to this CTA */
-    if (places > 0) {
-        const long long in = scan_s[W];
-        const int b = find_s, np = attn_places<F::BLOCK>(attn_keys(A, b)), item = (int)(in / np);
-        const int off = (int)(in - (long long)item * np);
-        to.set(A, b, item, max(off - kAttnItemCost, 0));
-        skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
-        places -= skipped;
-    }
     if (places <= 0) {
-        if (tid == 0 && !A.by_item) A.desc[part] = make_int2(-1, 0);
+        if (!whole_items && tid == 0 && !A.by_item) A.desc[part] = make_int2(-1, 0);
         return;
     }
     at = to;
-    bool began = at.blk == 0;                          /* this CTA holds the beginning of the item */
-    /* the item that ends here and began in an earlier CTA; which one it began in follows from the cut */
-    if (tid == 0) {
-        int2 d = make_int2(-1, 0);
-        if (!began && places >= at.nb - at.blk) {
-            const long long first = u0 + skipped - at.blk;       /* place of the item's first block */
-            int p = (int)(first * parts / total);
-            while (total * p / parts > first) p--;
-            while (total * (p + 1) / parts <= first) p++;
-            d = make_int2(A.by_item ? part : at.b * items + at.h, p);
-        }
-        if (!A.by_item) A.desc[part] = d;
-        else if (d.x >= 0) A.desc[at.b * items + at.h] = d;
-    }
+    bool began = at.blk == 0;                          /* this part holds the beginning of the item */
 
     /* What is copied next: units lane, lane + 32, .. of the group's rows. The pointers are those of the first
      * of them in row 0 of the cache. */
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         vlane = A.v_store + to.hk * F::VEC + lane_off;
     };
     auto aim = [&]() {                                 /* this warp's rows of block to.blk: never across a page */
-        const int at = to.blk * F::BLOCK + F::KEYS * warp;
+        const int at = to.blk * BLOCK + warp_key;
         row_to = -1;
         if (at < to.n) {
             if (A.block_table != nullptr) {
@@ -579,13 +579,14 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     aim_item();
     aim();
     int to_places = places;                            /* places from `to` on */
+    bool to_more = true;                               /* something is left to copy */
     const bool odd_end = TQ && (((size_t)A.n_slots * A.n_kv) & 1) != 0;      /* the last RMS value stands alone in its word */
     auto issue = [&](int stage) -> int {               /* returns how many of the warp's 16 rows hold keys */
         int live = 0;
-        if (to_places > 0) {
+        if (to_more) {
             const uint32_t base = ring + stage * S::STAGE, kd = base + lane_dst, md = base + 2 * S::ROWS + lane4;
             const int row0 = row_to;
-            live = row_to < 0 ? 0 : min(min(to.n - to.blk * F::BLOCK - F::KEYS * warp, A.n_slots - row0), F::KEYS);
+            live = row_to < 0 ? 0 : min(min(to.n - to.blk * BLOCK - warp_key, A.n_slots - row0), F::KEYS);
             if (live == F::KEYS && !(TQ && odd_end && row0 + F::KEYS >= A.n_slots)) {
                 const uint8_t* kp = klane + (size_t)(uint32_t)row0 * row_bytes;
                 const uint8_t* vp = vlane + (size_t)(uint32_t)row0 * row_bytes;
@@ -628,16 +629,17 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
             }
             live = max(live, 0);
             to_places--;
-            if (!to.last()) {
-                to.blk++;
-                if (to_places > 0) aim();
-            } else {
-                to_places -= kAttnItemCost;
-                if (to_places > 0) {
+            const bool ends = to.last();
+            to_more = whole_items ? !ends || to_places > 0 : to_places > (ends ? kAttnItemCost : 0);
+            if (to_more) {
+                if (ends) {
+                    to_places -= kAttnItemCost;
                     to.next_item(A, items);
                     aim_item();
-                    aim();
+                } else {
+                    to.blk++;
                 }
+                aim();
             }
         }
         cp_commit();
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     for (int s = 0; s < S::STAGES - 1; s++) live_q[s] = issue(s);
 
     uint32_t q[NT][HD / 8];
-    auto load_q = [&](const AttnAt<F::BLOCK>& x) {
+    auto load_q = [&](const AttnAt<BLOCK>& x) {
         const int h0 = (x.h - x.hk * A.head_blocks) * 8 * NT, heads = A.group - h0;      /* of this block: at most 8 NT */
         const __half* src = A.q + ((size_t)x.b * A.n_q + (size_t)x.hk * A.group + h0) * HD;
 #pragma unroll
@@ -672,6 +674,19 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     };
     load_q(at);
     begin_item();
+    /* the item that ends here and began in an earlier part; which one it began in follows from the cut */
+    if (!whole_items && tid == 0) {
+        int2 d = make_int2(-1, 0);
+        if (!began && places >= at.nb - at.blk) {
+            const long long first = u0 + skipped - at.blk;       /* place of the item's first block */
+            int p = min((int)((float)first / (float)total * (float)parts), part);
+            while (cut.at(p) > first) p--;
+            while (cut.at(p + 1) <= first) p++;
+            d = make_int2(A.by_item ? part : at.b * items + at.h, p);
+        }
+        if (!A.by_item) A.desc[part] = d;
+        else if (d.x >= 0) A.desc[at.b * items + at.h] = d;
+    }
 
     const uint32_t k_at = attn_k_at<FMT, HD>(lane), v_at = attn_v_at<FMT, HD>(lane);
     int stage = 0;
@@ -706,8 +721,8 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         /* the next item's Q is on its way while this one is finished */
         const bool item_done = at.last();
         places--;
-        const bool more = item_done ? places > kAttnItemCost : places > 0;
-        AttnAt<F::BLOCK> nx = at;
+        const bool more = whole_items ? !item_done || places > 0 : places > (item_done ? kAttnItemCost : 0);
+        AttnAt<BLOCK> nx = at;
         if (!item_done) {
             nx.blk++;
         } else if (more) {
@@ -841,9 +856,23 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
             }
         const int h0 = (at.h - at.hk * A.head_blocks) * 8 * NT, heads = A.group - h0;
         const size_t head0 = (size_t)at.b * A.n_q + (size_t)at.hk * A.group + h0;
-        const bool whole = began && item_done;
+        const bool whole = SOLO || (began && item_done);
         const int slot = 2 * part + (began ? 1 : 0);               /* an item that began here is this CTA's last */
-        if (A.by_item && whole && tid == 0) A.desc[at.b * items + at.h] = make_int2(-1, 0);
+        if (!whole_items && A.by_item && whole && tid == 0) A.desc[at.b * items + at.h] = make_int2(-1, 0);
+        if constexpr (SOLO) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int h = 8 * nt + 2 * t + c;
+                    if (h >= heads) continue;
+                    const float f = vref * (1.0f / attn_alpha<FMT>());
+#pragma unroll
+                    for (int j = 0; j < TILES; j++)
+                        attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(o[nt][j][c] * f, o[nt][j][c + 2] * f, l[nt][c]));
+                    if (A.lse != nullptr && g == 0) A.lse[head0 + h] = attn_lse(m[nt][c], l[nt][c]);
+                }
+        } else {
         /* each warp leaves its output in the stage that it has read last, which nothing is copied into before the
          * next step */
 #pragma unroll
@@ -907,6 +936,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
             }
         }
         __syncthreads();                               /* all has been read */
+        }
         if (!more) break;
         places -= kAttnItemCost;
         at = nx;
@@ -996,6 +1026,18 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
  * (head_dim 256: one, for the registers), the rest in further items of the same cache head. */
 static int attn_col_tiles(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 2 : 1; }
 
+/* Whether items stay whole, which saves the joining kernel: 2, each a warp's; 1, each a CTA's; 0, they are cut. By
+ * the positions that a sequence can have, since its length is known on the device alone. Measured with every
+ * sequence as long as that, 28 heads over 4 of 128 in FP16, us (cut / CTA / warp):
+ *   1 sequence     64: 5.4 / 4.5 / 5.6    200: 6.9 / 6.5 / 11.0    500: 7.3 / 9.2 / 22.5
+ *   32            200: 9.6 / 7.3 / 12.5   500: 13.3 / 13.0 / 28.5  1000: 20.1 / 20.9 / 54.3
+ *   96             64: 8.4 / 6.4 / 6.6    500: 25.5 / 20.1 / 33.4  1000: 39.7 / 34.3 / 60.4
+ *   300            64: 18.7 / 16.7 / 12.9 200: 31.7 / 27.5 / 26.1  1000: 102 / 96.8 / 96.8 */
+static int attn_whole(long long items, long long capacity) {
+    if (items >= 888 && capacity <= 256) return 2;
+    return capacity <= 256 || (items > 128 && capacity <= 512) || (items >= 384 && capacity <= 1024) ? 1 : 0;
+}
+
 struct AttnScratch { size_t ml, o, bytes; };
 static AttnScratch attn_scratch(int group, int head_dim) {
     const size_t heads = 8 * (size_t)attn_col_tiles(group, head_dim);
@@ -1011,22 +1053,29 @@ static cudaError_t launch_attn(AttnArgs A, cudaStream_t s) {
     constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM, parts = AttnShape<FMT, HD, NT>::CTAS * kAttnSms;
     static_assert(parts <= kAttnParts, "the scratch holds kAttnParts parts");
     A.parts = parts;
-    cudaError_t e = cudaFuncSetAttribute((const void*)attn_decode_kernel<FMT, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    const bool solo = A.whole_items == 2;
+    cudaError_t e = cudaFuncSetAttribute(solo ? (const void*)attn_decode_kernel<FMT, HD, NT, true> : (const void*)attn_decode_kernel<FMT, HD, NT, false>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     /* Even parts want evenly filled SMs. A CTA that is placed while the kernel before still holds some of them
      * starts where there is room, and its part ends late (64 x 4096: 107 us instead of 86, behind a kernel of 888
      * small CTAs), so this is an ordinary launch unless there are few items: then the launch itself is what counts. */
-    if (A.by_item) {
-        e = launch_pdl(attn_decode_kernel<FMT, HD, NT>, dim3(parts), dim3(32 * AttnFmt<FMT, HD>::W), (size_t)SMEM, s, A);
+    const dim3 block(32 * AttnFmt<FMT, HD>::W);
+    if (solo) {
+        e = launch_pdl(attn_decode_kernel<FMT, HD, NT, true>, dim3(parts), block, (size_t)SMEM, s, A);
+    } else if (A.by_item || A.whole_items) {
+        e = launch_pdl(attn_decode_kernel<FMT, HD, NT, false>, dim3(parts), block, (size_t)SMEM, s, A);
     } else {
-        attn_decode_kernel<FMT, HD, NT><<<dim3(parts), dim3(32 * AttnFmt<FMT, HD>::W), (size_t)SMEM, s>>>(A);
+        attn_decode_kernel<FMT, HD, NT, false><<<dim3(parts), block, (size_t)SMEM, s>>>(A);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (A.whole_items) return e;
     constexpr int TILES = NT * (HD / 16);
     if (A.by_item) e = launch_pdl(attn_join_kernel<FMT, HD, NT, 8>, dim3(A.n_seqs * A.n_kv * A.head_blocks, TILES), dim3(256), 0, s, A);
     else e = launch_pdl(attn_join_kernel<FMT, HD, NT, 4>, dim3((parts + kAttnJoinParts - 1) / kAttnJoinParts, TILES), dim3(128), 0, s, A);
-    if (e == cudaSuccess) g_launches.fetch_add(2, std::memory_order_relaxed);
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }
 template <int FMT>
@@ -1055,12 +1104,15 @@ extern "C" int vvbk_attn_decode(const void* q, void* out, float* lse, const void
     const int group = n_q_heads / n_kv_heads, nt = attn_col_tiles(group, head_dim);
     const AttnScratch sc = attn_scratch(group, head_dim);
     uint8_t* const base = (uint8_t*)scratch;
+    const int head_blocks = (group + 8 * nt - 1) / (8 * nt);
+    const long long items = (long long)n_seqs * n_kv_heads * head_blocks;
+    const long long capacity = block_table != nullptr ? (long long)table_stride << kAttnPageShift : (long long)table_stride;
+    const int whole = attn_whole(items, capacity);
     const AttnArgs A = {(const __half*)q, (__half*)out, lse, (const uint8_t*)k_store, (const uint8_t*)v_store,
                         (const __half*)k_meta, (const __half*)v_meta, block_table, lens,
                         (int2*)base, (float2*)(base + sc.ml), (float4*)(base + sc.o),
                         n_seqs, n_q_heads, n_kv_heads, n_slots, table_stride, len_add,
-                        group, (group + 8 * nt - 1) / (8 * nt),
-                        0, (long long)n_seqs * n_kv_heads * ((group + 8 * nt - 1) / (8 * nt)) <= kAttnFewItems, scale * kLog2e};
+                        group, head_blocks, 0, items <= kAttnFewItems, whole, scale * kLog2e};
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
     switch (kv_format) {
