@@ -494,7 +494,10 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     }
     const long long total = __shfl_sync(0xffffffffu, upto, 31) * items, before = (upto - mine) * items;
     const int part = SOLO ? blockIdx.x * W + warp : blockIdx.x;
-    const int parts = (int)max(min((long long)(SOLO ? gridDim.x * W : gridDim.x), total / (1 + kAttnItemCost)), 1ll);
+    /* as few parts as make the largest no larger: 908 places on 444 CTAs are 303 parts of three, not 444 of two or three */
+    const unsigned most = SOLO ? gridDim.x * W : gridDim.x;
+    const long long largest = max(total <= 0x7fffffffll ? (long long)(((unsigned)total + most - 1) / most) : (total + most - 1) / most, 1ll + kAttnItemCost);
+    const int parts = (int)max(total <= 0x7fffffffll ? (long long)(((unsigned)total + (unsigned)largest - 1) / (unsigned)largest) : (total + largest - 1) / largest, 1ll);
     const AttnCut cut(total, parts);
     const long long u0 = part < parts ? cut.at(part) : total, u1 = part < parts ? cut.at(part + 1) : total;
 
