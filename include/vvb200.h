@@ -354,6 +354,7 @@ vv_status_t vvb_kv_unrotate_dev(void* x_fp16, int n_heads, int head_dim, int row
  *  max_rows. Sequences are admitted in order: one is refused for pages when the
  *  pages asked for up to and including it exceed the stack's height, so a later
  *  sequence is never admitted in an earlier one's place unless it needs none.
+ *  A page belongs to one sequence: what two tables name is pushed twice.
  *  lens_out may be lens and free_count_out may be free_count; no other two
  *  arrays may overlap. Table entries beyond a sequence's pages are not touched.
  *  The result does not depend on timing. 1 <= table_stride <= 2^25 - 1, n_pages
@@ -424,7 +425,7 @@ vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* args, void* str
  *  A reference key (k_ref) shifts all scores of a head alike and is not needed.
  *  head_dim 64, 128 or 256 (TurboQuant: 128); n_q_heads a multiple of n_kv_heads;
  *  q, out, the stores and scratch 16-byte aligned, k_meta and v_meta 4-byte
- *  aligned (VV_ERR_UNSUPPORTED otherwise); n_seqs <= 8192. out may be q. scratch:
+ *  aligned (VV_ERR_UNSUPPORTED otherwise); n_seqs <= 8192, n_q_heads <= 4096. out may be q. scratch:
  *  vvb_attn_decode_scratch_bytes(...) bytes of device memory whose contents need
  *  no initialisation; calls that overlap on a GPU need one each (two captured
  *  graphs may share one when they do not run at the same time). The work is

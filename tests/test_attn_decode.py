@@ -35,7 +35,7 @@ def fake(vv, **kw):
     (dict(kv_format=TQ4, head_dim=64, k_meta=P, v_meta=P), "VV_ERR_UNSUPPORTED"), (dict(kv_format=TQ4, k_meta=P + 2, v_meta=P), "VV_ERR_UNSUPPORTED"),
     (dict(q=P + 8), "VV_ERR_UNSUPPORTED"), (dict(k_store=P + 4), "VV_ERR_UNSUPPORTED"), (dict(scratch=P + 8), "VV_ERR_UNSUPPORTED"),
     (dict(lens=P + 2), "VV_ERR_INVALID_ARG"), (dict(block_table=P + 2), "VV_ERR_INVALID_ARG"), (dict(lse=P + 1), "VV_ERR_INVALID_ARG"),
-    (dict(table_stride=1 << 25), "VV_ERR_OVERFLOW"), (dict(n_seqs=8193), "VV_ERR_UNSUPPORTED"), (dict(scratch_bytes=0), "VV_ERR_INVALID_ARG"),
+    (dict(n_q_heads=8192), "VV_ERR_UNSUPPORTED"), (dict(table_stride=1 << 25), "VV_ERR_OVERFLOW"), (dict(n_seqs=8193), "VV_ERR_UNSUPPORTED"), (dict(scratch_bytes=0), "VV_ERR_INVALID_ARG"),
     (dict(n_seqs=0), "VV_OK"),
 ])
 def test_attn_refusals(lib, kw, want):
@@ -201,6 +201,46 @@ def test_attn_rotated_formats_head_layouts(vv, nq, nkv, fmt):
 def test_attn_long_and_many(vv, lens, fmt, paged):
     c = Case(vv, lens, 28 if len(lens) < 200 else 8, 4, 128, fmt, paged, seed=len(lens)).upload()
     c.check(*c.run())
+
+
+# by the positions a table has room for and the number of sequences the work is cut differently: whole sequences to
+# warps or to CTAs, or cut between CTAs with their pieces found by item or by CTA
+WAYS = {"warps": (250, 250, 64), "warps_edge": (222, 256, 0), "ctas": (100, 500, 0), "ctas_few": (2, 190, 64), "ctas_many": (97, 1000, 0),
+        "cut_few": (5, 900, 64), "cut_nine": (9, 2500, 0), "cut": (20, 3000, 64), "cut_many": (300, 1100, 0)}
+
+
+@gpu
+@pytest.mark.parametrize("fmt", range(7))
+@pytest.mark.parametrize("way", WAYS)
+def test_attn_every_way_of_cutting_the_work(vv, way, fmt):
+    n, top, room = WAYS[way]
+    rng = np.random.default_rng(n + fmt)
+    lens = np.where(rng.random(n) < 0.1, 0, np.exp(rng.uniform(0, np.log(top + 1), n))).astype(np.int64)
+    lens[rng.integers(n)] = top
+    c = Case(vv, lens, 16, 4, 128, fmt, seed=n, slack=room // 64).upload()
+    n0 = vv.launch_count()
+    out, lse = c.run()
+    assert vv.launch_count() - n0 == (2 if way.startswith("cut") else 1)
+    c.check(out, lse)
+    again = c.run()
+    assert np.array_equal(again[0], out) and np.array_equal(again[1], lse)
+
+
+@gpu
+def test_attn_nothing_but_empty_sequences(vv):
+    for n, room in ((1, 1), (5, 40), (1000, 1)):
+        c = Case(vv, [0] * n, 28, 4, 128, FP16, seed=n, slack=room).upload()
+        c.check(*c.run())
+
+
+@gpu
+def test_attn_contiguous_cache_shorter_than_its_sequences_claim(vv):
+    """Lengths beyond the rows that the cache has: cut there, nothing beyond is read."""
+    c = Case(vv, [300, 200], 4, 2, 128, FP16, paged=False, seed=21, slack=0).upload()
+    c.dlens.copy_(torch.tensor([2 ** 31 - 1, 2 ** 31 - 1], dtype=torch.int32))
+    c.args.n_slots = 500                                # the second sequence's stretch ends after 200
+    out, lse = c.run()
+    c.check(out, lse)
 
 
 @gpu

@@ -51,16 +51,6 @@ namespace vvb {
 extern std::atomic<uint64_t> g_launches;
 
 constexpr int kAttnPageShift = 6;
-#ifndef VVB_ATTN_KG
-#define VVB_ATTN_KG (VEC >= 256 ? 1 : VEC >= 64 ? 2 : 4)
-#endif
-#ifndef VVB_ATTN_WARPS
-#define VVB_ATTN_WARPS(FMT, HD) 4
-#endif
-#ifndef VVB_ATTN_CTAS
-#define VVB_ATTN_CTAS(FMT, HD, NT) (HD == 256 || NT == 2 ? 2 : 3)
-#define VVB_ATTN_STAGES(FMT, HD, NT) (FMT == KV_TQ4 || AttnFmt<FMT, HD>::VEC * AttnFmt<FMT, HD>::KG >= 256 ? 2 : 3)
-#endif
 constexpr int kAttnSms = 148, kAttnParts = 3 * kAttnSms;      /* parts the work is cut into, at most */
 constexpr int kAttnFewItems = 37;               /* so many items, in eight tiles each, are one wave of the joining kernel */
 constexpr int kAttnJoinParts = 4, kAttnJoinChunk = 4;
@@ -99,13 +89,14 @@ template <int FMT, int HD> struct AttnFmt {
     static constexpr int VEC = kv_is_tq(FMT) ? tq_bytes_per_vec(FMT) : FMT == KV_RAW ? 2 * HD : HD;
     static constexpr bool MAT = FMT != KV_TQ3 && FMT != KV_TQ1_5;
     static constexpr int UNIT = FMT == KV_TQ1_5 ? 8 : 16;
-    static constexpr int KG = VVB_ATTN_KG;                       /* groups a warp takes in a step; the warps' groups are a block */
-    static constexpr int W = VVB_ATTN_WARPS(FMT, HD);            /* warps of a CTA */
+    static constexpr int KG = VEC >= 256 ? 1 : VEC >= 64 ? 2 : 4;                     /* groups a warp takes in a step; the warps' groups are a block */
+    static constexpr int W = FMT == KV_TQ4 ? 12 : 4;             /* warps of a CTA; the 4-bit code table is for many */
     static constexpr int KEYS = 16 * KG, BLOCK = W * KEYS;
     static constexpr int PER_ROW = VEC / UNIT, UNITS = KEYS * PER_ROW, COPIES = (UNITS + 31) / 32;    /* of a step, copies a lane makes */
     /* dims of a word that ldmatrix brings: of K a lane's 4 bytes, of V the 2 bytes of one key */
     static constexpr int K_DIMS = FMT == KV_RAW ? 2 : FMT == KV_TQ4 ? 8 : FMT == KV_TQ2 ? 16 : 4;
     /* entries of the code table: two codes -> two levels; 1.5 bits: code -> pair, then two keys' codes -> two pairs */
+    static constexpr int LUT_STEP = FMT == KV_TQ4 ? 256 : 128;   /* bytes from entry to entry: 32 lanes' copies, and room */
     static constexpr int LUT = FMT == KV_TQ4 ? 256 : FMT == KV_TQ3 ? 64 : FMT == KV_TQ2 ? 16 : FMT == KV_TQ1_5 ? 8 + 128 : 0;
 };
 
@@ -120,12 +111,12 @@ template <int FMT, int HD, int NT> struct AttnShape {
     static constexpr int USED = 2 * ROWS + (kv_is_tq(FMT) ? 8 * F::KEYS : 0);                 /* then the words that hold the rows' RMS values */
     static constexpr int OUT = NT * HD * 32;                                                  /* a warp's output, left in the stage it has read last */
     static constexpr int STAGE = USED > OUT ? USED : OUT;
-    static constexpr int CTAS = VVB_ATTN_CTAS(FMT, HD, NT);                                   /* an SM's, by registers and shared memory */
-    static constexpr int STAGES = VVB_ATTN_STAGES(FMT, HD, NT);
+    static constexpr int CTAS = F::W == 12 ? 1 : HD == 256 || NT == 2 ? 2 : 3;                /* an SM's, by registers and shared memory */
+    static constexpr int STAGES = FMT == KV_TQ4 || F::VEC * F::KG >= 256 ? 2 : 3;
     static constexpr int RING = STAGE * STAGES;                                               /* a warp's */
     static constexpr int TILES = HD / 16;                                                     /* 16-dim tiles of the output */
-    static constexpr int MINE = NT * TILES / F::W;                                            /* of them a warp finishes */
-    static constexpr int LUT = F::LUT * 128;
+    static constexpr int MINE = (NT * TILES + F::W - 1) / F::W;                               /* of them a warp finishes */
+    static constexpr int LUT = F::LUT * F::LUT_STEP;
     static constexpr int SMEM = LUT + F::W * RING;                                            /* in this order */
 };
 
@@ -210,6 +201,11 @@ __device__ __forceinline__ uint32_t attn_lut(uint32_t c, uint32_t mask, uint32_t
     return *reinterpret_cast<const uint32_t*>(attn_smem + from + ((c & mask) | lane4));
 }
 
+/* The same for byte k of w, entries 256 bytes apart: one byte permute puts the byte above the lane's offset. */
+__device__ __forceinline__ uint32_t attn_lut_byte(uint32_t w, int k, uint32_t lane4) {
+    return *reinterpret_cast<const uint32_t*>(attn_smem + __byte_perm(w, lane4, 0x7704 + (k << 4)));
+}
+
 /* ---------------------------------------------------------------- code books */
 
 __constant__ float c_lev4[16] = {tq_lev4(0), tq_lev4(1), tq_lev4(2), tq_lev4(3), tq_lev4(4), tq_lev4(5), tq_lev4(6), tq_lev4(7),
@@ -258,7 +254,7 @@ template <int FMT> __device__ __forceinline__ int attn_v_dim(int e, int g) {
 
 /* Two dims' codes at bit `bit` of words w -> two halves. */
 template <int FMT> __device__ __forceinline__ uint32_t attn_decode2(const uint32_t* w, int bit, uint32_t lane4) {
-    constexpr int NB = FMT == KV_TQ4 ? 8 : FMT == KV_TQ3 ? 6 : FMT == KV_TQ2 ? 4 : 3;
+    constexpr int NB = FMT == KV_TQ3 ? 6 : FMT == KV_TQ2 ? 4 : 3;
     const int at = bit & 31;
     uint32_t c;                                        /* the codes times 128 */
     if (at + NB > 32) c = __funnelshift_r(w[bit >> 5], w[(bit >> 5) + 1], at) << 7;
@@ -288,8 +284,8 @@ __device__ __forceinline__ void attn_load_k(uint32_t a, int t, uint32_t (&lo)[HD
                 } else {
 #pragma unroll
                     for (int x = 0; x < W; x++) {
-                        lo[i + x] = attn_decode2<FMT>(&w[2 * k], 32 / W * x, lane4);
-                        hi[i + x] = attn_decode2<FMT>(&w[2 * k + 1], 32 / W * x, lane4);
+                        lo[i + x] = FMT == KV_TQ4 ? attn_lut_byte(w[2 * k], x, lane4) : attn_decode2<FMT>(&w[2 * k], 32 / W * x, lane4);
+                        hi[i + x] = FMT == KV_TQ4 ? attn_lut_byte(w[2 * k + 1], x, lane4) : attn_decode2<FMT>(&w[2 * k + 1], 32 / W * x, lane4);
                     }
                 }
             }
@@ -332,13 +328,13 @@ __device__ __forceinline__ void attn_load_v(uint32_t a, int g, uint32_t (&xa)[HD
                 } else if constexpr (!kv_is_tq(FMT)) {
                     fp8_halves<FMT, true>(w[k], x[2 * c], x[2 * c + 1]);
                 } else if constexpr (FMT == KV_TQ4) {
-                    uint32_t even = w[k] & 0x0f0f0f0fu, odd = (w[k] >> 4) & 0x0f0f0f0fu;      /* A0 A2 B0 B2, A1 A3 B1 B3 */
-                    even |= even >> 12;                /* bytes 0, 1: A0 B0, A2 B2 */
-                    odd |= odd >> 12;
-                    x[4 * c] = attn_lut(even << 7, 0x7f80u, lane4);
-                    x[4 * c + 1] = attn_lut(odd << 7, 0x7f80u, lane4);
-                    x[4 * c + 2] = attn_lut(even >> 1, 0x7f80u, lane4);
-                    x[4 * c + 3] = attn_lut(odd >> 1, 0x7f80u, lane4);
+                    /* A's dims 0, 1 and 2, 3 of the four, B's: pairs by dim, then interleaved */
+                    const uint32_t a0 = attn_lut_byte(w[k], 0, lane4), a1 = attn_lut_byte(w[k], 1, lane4);
+                    const uint32_t b0 = attn_lut_byte(w[k], 2, lane4), b1 = attn_lut_byte(w[k], 3, lane4);
+                    x[4 * c] = __byte_perm(a0, b0, 0x5410);
+                    x[4 * c + 1] = __byte_perm(a0, b0, 0x7632);
+                    x[4 * c + 2] = __byte_perm(a1, b1, 0x5410);
+                    x[4 * c + 3] = __byte_perm(a1, b1, 0x7632);
                 } else {
                     uint32_t even = w[k] & 0x33333333u, odd = (w[k] >> 2) & 0x33333333u;      /* every other code, A's in the low half */
                     even |= even >> 14;                /* fields of 4 bits: A0 B0, A2 B2, .. */
@@ -408,11 +404,12 @@ template <int FMT> __device__ __forceinline__ void attn_store(__half* out, int j
 
 /* ---------------------------------------------------------------- work */
 
-/* Number of keys of sequence b. */
+/* Number of keys of sequence b: no more than its table, or its stretch of the contiguous cache, has places for. */
 __device__ __forceinline__ int attn_keys(const AttnArgs& A, int b) {
-    const long long cap = A.block_table != nullptr ? (long long)A.table_stride << kAttnPageShift : (long long)A.table_stride;
+    const long long cap = A.block_table != nullptr ? (long long)A.table_stride << kAttnPageShift
+                                                   : min((long long)A.table_stride, (long long)A.n_slots - (long long)b * A.table_stride);
     const long long n = (long long)__ldg(A.lens + b) + A.len_add;
-    return (int)min(min(max(n, 0ll), cap), 0x7fffff00ll);
+    return (int)max(min(min(n, cap), 0x7fffff00ll), 0ll);
 }
 template <int BLOCK> __device__ __forceinline__ int attn_blocks(int n) { return (int)(((unsigned)n + (BLOCK - 1)) / BLOCK); }
 template <int BLOCK> __device__ __forceinline__ int attn_places(int n) { return n > 0 ? attn_blocks<BLOCK>(n) + kAttnItemCost : 0; }
@@ -471,7 +468,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     const uint32_t lane4 = 4 * lane;                   /* this lane's copy of the table */
 
     if constexpr (F::LUT > 0) {
-        for (int e = warp; e < F::LUT; e += W) *reinterpret_cast<uint32_t*>(attn_smem + 128 * e + lane4) = attn_lut_entry<FMT>(e);
+        for (int e = warp; e < F::LUT; e += W) *reinterpret_cast<uint32_t*>(attn_smem + F::LUT_STEP * e + lane4) = attn_lut_entry<FMT>(e);
         if (SOLO) __syncthreads();
     }
     pdl_wait();
@@ -897,7 +894,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         }
         if (lane == 0) f_s[warp] = vref;
         __syncthreads();
-        {
+        if (warp * MINE < NT * TILES) {
             const int nt = warp * MINE / TILES;        /* a warp's tiles are of one column tile */
             float top[2], sum[2], f[W][2];
 #pragma unroll
@@ -1028,9 +1025,9 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
     }
 }
 
-/* Column tiles of 8 query heads an item holds: two where the group has more than eight heads
- * (head_dim 256: one, for the registers), the rest in further items of the same cache head. */
-static int attn_col_tiles(int group, int head_dim) { return group > 8 && head_dim <= 128 ? 2 : 1; }
+/* Column tiles of 8 query heads an item holds: two where the group has more than eight heads (one for 256-wide heads,
+ * by registers, and for the 4-bit format, by shared memory), the rest in further items of the same cache head. */
+static int attn_col_tiles(int group, int head_dim, int fmt) { return group > 8 && head_dim <= 128 && fmt != KV_TQ4 ? 2 : 1; }
 
 /* Whether items stay whole, which saves the joining kernel: 2, each a warp's; 1, each a CTA's; 0, they are cut. By
  * the positions that a sequence can have, since its length is known on the device alone. Measured with every
@@ -1046,7 +1043,7 @@ static int attn_whole(long long items, long long capacity) {
 
 struct AttnScratch { size_t ml, o, bytes; };
 static AttnScratch attn_scratch(int group, int head_dim) {
-    const size_t heads = 8 * (size_t)attn_col_tiles(group, head_dim);
+    const size_t heads = group > 8 && head_dim <= 128 ? 16 : 8;          /* of an item, whatever the format */
     AttnScratch s;
     s.ml = kAttnParts * sizeof(int2);                                   /* 16-byte multiples */
     s.o = s.ml + 2 * kAttnParts * heads * sizeof(float2);
@@ -1090,7 +1087,12 @@ static cudaError_t launch_attn(const AttnArgs& A, int head_dim, int nt, cudaStre
         if (head_dim == 64) return nt == 2 ? launch_attn<FMT, 64, 2>(A, s) : launch_attn<FMT, 64, 1>(A, s);
         if (head_dim == 256) return launch_attn<FMT, 256, 1>(A, s);
     }
-    if (head_dim == 128) return nt == 2 ? launch_attn<FMT, 128, 2>(A, s) : launch_attn<FMT, 128, 1>(A, s);
+    if (head_dim == 128) {
+        if constexpr (FMT != KV_TQ4) {
+            if (nt == 2) return launch_attn<FMT, 128, 2>(A, s);
+        }
+        return launch_attn<FMT, 128, 1>(A, s);
+    }
     return cudaErrorNotSupported;
 }
 
@@ -1107,7 +1109,7 @@ extern "C" int vvbk_attn_decode(const void* q, void* out, float* lse, const void
                                 const void* k_meta, const void* v_meta, const int* block_table, const int* lens,
                                 void* scratch, int n_seqs, int n_q_heads, int n_kv_heads, int head_dim, int n_slots,
                                 int table_stride, int len_add, int kv_format, float scale, void* stream) {
-    const int group = n_q_heads / n_kv_heads, nt = attn_col_tiles(group, head_dim);
+    const int group = n_q_heads / n_kv_heads, nt = attn_col_tiles(group, head_dim, kv_format);
     const AttnScratch sc = attn_scratch(group, head_dim);
     uint8_t* const base = (uint8_t*)scratch;
     const int head_blocks = (group + 8 * nt - 1) / (8 * nt);

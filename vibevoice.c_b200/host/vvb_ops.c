@@ -111,6 +111,7 @@ vv_status_t vvb_kv_append_dev(const vvb_kv_append_t* a, void* stream) {
 
 #define VVB_MAX_PAGES ((1 << 25) - 1)     /* positions and cache rows stay below 2^31 */
 #define VVB_MAX_SEQS 8192
+#define VVB_MAX_HEADS 4096
 
 vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* a, void* stream) {
     if (!a) return VV_ERR_NULL_PTR;
@@ -173,7 +174,7 @@ vv_status_t vvb_attn_decode_dev(const vvb_attn_decode_t* a, void* stream) {
     if (tq && (!a->k_meta || !a->v_meta)) return VV_ERR_NULL_PTR;
     if (a->head_dim != 128 && (tq || (a->head_dim != 64 && a->head_dim != 256))) return VV_ERR_UNSUPPORTED;
     if (a->block_table && a->table_stride > VVB_MAX_PAGES) return VV_ERR_OVERFLOW;
-    if (a->n_seqs > VVB_MAX_SEQS) return VV_ERR_UNSUPPORTED;
+    if (a->n_seqs > VVB_MAX_SEQS || a->n_q_heads > VVB_MAX_HEADS) return VV_ERR_UNSUPPORTED;
     const void* wide[] = {a->q, a->out, a->k_store, a->v_store, a->scratch};
     for (size_t i = 0; i < sizeof wide / sizeof wide[0]; i++)
         if ((uintptr_t)wide[i] & 15u) return VV_ERR_UNSUPPORTED;
