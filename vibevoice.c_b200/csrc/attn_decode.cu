@@ -419,7 +419,7 @@ template <int BLOCK> struct AttnAt {
     __device__ __forceinline__ void set(const AttnArgs& A, int seq, int item, int block) {
         b = seq;
         h = item;
-        hk = h / A.head_blocks;
+        hk = A.head_blocks == 1 ? h : h / A.head_blocks;
         blk = block;
         n = attn_keys(A, b);
         nb = attn_blocks<BLOCK>(n);
@@ -429,7 +429,7 @@ template <int BLOCK> struct AttnAt {
     __device__ __forceinline__ void next_item(const AttnArgs& A, int items) {
         blk = 0;
         if (++h < items) {
-            hk = h / A.head_blocks;
+            hk = A.head_blocks == 1 ? h : h / A.head_blocks;
             return;
         }
         h = hk = 0;
