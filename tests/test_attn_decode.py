@@ -292,6 +292,42 @@ def test_attn_tail_of_tiny_weights(vv):
 
 
 @gpu
+@pytest.mark.parametrize("depth", [26.0, 50.0, 200.0])
+def test_attn_weights_too_small_to_matter_do_not_add_up(vv, depth):
+    """A hundred thousand keys far below the largest, with values near FP16's largest."""
+    n = 100_000
+    c = Case(vv, [n], 1, 1, 128, FP16, seed=9)
+    s = c.slots(0)
+    k, v = (x.view(np.float16).reshape(c.rows, 128) for x in c.kv)
+    k[s] = 0
+    v[s] = 60000.0
+    k[s[n // 3], 0], v[s[n // 3]] = depth * 11.3125, 1.0
+    c.q[:] = 0
+    c.q[0, 0, 0] = 1.0
+    c.upload()
+    c.check(*c.run())
+
+
+@gpu
+def test_attn_infinite_values(vv):
+    """An infinity in V stays one where its key has weight, with any sign of the values around it."""
+    c = Case(vv, [90, 300], 8, 2, 128, FP16, seed=22)
+    v = c.kv[1].view(np.float16).reshape(c.rows, 2, 128)
+    s = c.slots(1)
+    v[s[::7], 0, 5] = np.inf
+    v[s[::11], 1, 100] = -np.inf
+    c.upload()
+    out, lse = c.run()
+    assert np.isposinf(out[1, :4, 5]).all() and np.isneginf(out[1, 4:, 100]).all() and np.isfinite(out).sum() == out.size - 8
+    v[s[::7], 0, 5], v[s[::11], 1, 100] = 0.0, 0.0
+    out[1, :4, 5], out[1, 4:, 100] = 0.0, 0.0
+    for h, d in [(h, 5) for h in range(4)] + [(h, 100) for h in range(4, 8)]:
+        kk, vw = (_paged.decode(x[s], None, FP16, 128) for x in c.kv)
+        out[1, h, d] = _paged.attention(c.q[1].astype(np.float64), kk, vw, c.scale)[0][h, d]
+    c.check(out, lse)
+
+
+@gpu
 def test_attn_infinite_scores(vv):
     """A key whose score is -inf has no weight; where every key's is, the row is empty: zeros and -inf. +inf and NaN
     in a live key give NaN, and only in the heads and sequences that see it."""

@@ -10,33 +10,60 @@
  * conversions, few for the tensor cores. So both products run on mma.m16n8k16
  * with the KEYS (or the head's dims) as the 16 rows and the query heads as the 8
  * columns, S^T = K Q^T and O^T = V^T P^T: 7 of 8 columns carry work, where heads
- * as rows would waste nine of sixteen. (tcgen05 wants 64 rows and its operands
- * in shared memory behind barriers; at the rate HBM delivers, mma.sync is idle
- * nine tenths of the time.)
+ * as rows would waste nine of sixteen. (tcgen05 wants 64 rows at least, both
+ * operands of a product at hand behind barriers, and the weights back through
+ * shared memory; at the rate HBM delivers, the tensor pipe of this kernel is
+ * busy 14 % of the time in FP16, 28 % in FP8.)
  *
- * No data crosses lanes through shared memory. A contraction may take its terms
- * in any order, so each lane's share of a fragment is chosen to be what 16-byte
- * loads of one row bring: of K, row `lane / 4` (and + 8) of the group, 16 bytes
- * at 16 (lane % 4) of each 64; of V, rows 2t, 2t+1, 2t+8, 2t+9 (t = lane % 4),
- * 16 bytes at 16 (lane / 4) of each 128, the pairs of rows interleaved by byte
- * permutes. A lane copies its own bytes with cp.async into its own 16-byte
- * column of the warp's ring and reads them back itself: waiting for its own
- * copies is all the synchronisation there is, warps never wait for one another,
- * and three stages of 8 KB a warp are in flight without holding registers.
+ * A warp takes 16 keys of one cache head at a time (two or four such groups a
+ * step where rows are short). It copies their rows with cp.async into a ring of
+ * its own, whole rows by neighbouring lanes: a request to L2 is then a whole
+ * 128-byte line. (With each lane copying just the 16-byte pieces that its own
+ * fragments need, which takes no data across lanes at all, requests are half
+ * lines, and 64 x 4096 FP16 took 122.8 us, compute or no compute, instead of
+ * 91.5.) The 16-byte pieces of a row lie permuted by bits of its number, so that
+ * ldmatrix reads eight rows from eight banks; V through its transposing form,
+ * which makes it the product's operand as it is. Between warps there is no
+ * synchronisation until an item (a sequence's cache head) ends.
  *
- * Work: the 64-position blocks of all (sequence, cache head) items in one line,
- * cut into as many equal parts as there are CTAs (two an SM). The cut depends on
- * the lengths alone, which every CTA sums up on the device. The CTA's four warps
- * take a quarter of each block. An item that a CTA holds whole is finished by
- * it; of one that is cut, each CTA leaves its part (running maximum, sum, output)
- * in scratch and a second small kernel joins them in CTA order.
+ * FP8: e4m3 by cvt, two to an instruction; e5m2 is the upper half of an FP16
+ * value and needs one byte permute. TurboQuant: two codes index a table in
+ * shared memory of two FP16 levels, a copy for each lane, so that 32 lanes never
+ * meet in a bank. 16 keys of the 4-bit format are 406 instructions a warp, 70 of
+ * them such look-ups (FP16: about 220): it is issue-bound, its ALU pipe first
+ * (tried: entries 128 bytes apart, three CTAs of four warps with a table each:
+ * 61.6 us for 48 sequences of 4100 - 8200; 256 apart, where one byte permute
+ * forms the address, and twelve warps over one table: 58.9; fourteen and sixteen
+ * warps of fewer registers: 69, 84).
  *
- * Precision: scores, maximum, sums and outputs in FP32. A weight e^(s - m) goes
- * to the tensor cores as a pair of FP16 values, rounded-down head plus rest, times 2^15: one
- * FP16 value alone would add an error as large as the output's own rounding.
- * Both are kept positive, so that an infinity in V stays one. For the rotated
+ * Work: the blocks of 64 (128, 256, 384) positions of all items in one line, cut
+ * into equal parts, one for each CTA that fits the GPU at once. The cut depends
+ * on the lengths alone, which every warp sums up on the device, so the same
+ * inputs give the same bits. The CTA's warps share each block. An item that a
+ * CTA holds whole is finished by it, the warps' outputs exchanged in the ring's
+ * stage read last; of one that is cut, each CTA leaves its part (running maximum,
+ * sum, output) in scratch and a second kernel joins them. attn_way says when
+ * items stay whole instead and the second kernel is saved.
+ *
+ * Measured (28 heads over 4, 128 wide; GB/s of K and V): 64 x 4096 FP16 85.8 us
+ * = 6.26 TB/s, 0.95 of the device's copy rate; 96 sequences of 1 .. 16384 57.6 us,
+ * 0.85; 48 of 4100 .. 8200 in FP8 53.5 us, 0.85; the same in 4 bits 58.9 us, 0.40;
+ * 1 x 14449 FP16 12.6 us, latency: the first loads behind lens and table, three
+ * steps, and the join. Bytes in flight: one stage of 8 KB for each of 12 warps an
+ * SM beside the one being read; two stages are slower (89.4 us for 64 x 4096),
+ * and so are two CTAs an SM (88.3).
+ * A cluster of eight CTAs for an item, joined through distributed shared memory
+ * in one launch, costs more than the second kernel (1 x 300: 8.4 us, 7.1).
+ *
+ * Precision: scores, maximum, sums and outputs in FP32. A weight e^(s - m), times
+ * 2^12, goes to the tensor cores as a pair of FP16 values, the one rounded toward
+ * zero and the rest: one FP16 value alone would add an error as large as the
+ * output's own rounding. Where a weight matters both are positive (weight_rest), so
+ * that an infinity in V stays one; below 2^-37 of the largest it is nothing. The maximum follows the scores only beyond a factor of 2^3 (8 % of
+ * the steps instead of 41 % for normal scores over 600 keys): 2^15 is the largest
+ * weight then. For the rotated
  * formats the levels times a common factor become FP16 values within 9e-5 of
- * themselves (alpha below, found by trying factors in [1, 2); 1.6e-4 for the
+ * themselves (attn_alpha, found by trying factors in [1, 2); 1.6e-4 for the
  * 1.5-bit code words), the RMS of a key multiplies its score, the RMS of V the
  * weight, relative to a power of two that follows the largest RMS.
  */
@@ -149,8 +176,12 @@ __device__ __forceinline__ uint32_t pack2_rz(float a, float b) {       /* two ha
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
-__device__ __forceinline__ uint32_t hmax2_bits(uint32_t a, uint32_t b) {
-    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+/* The rest of two weights whose heads are `hi`: at least 2^-24 where the head is 2^-8 or more, so that an infinity in V
+ * meets two positive factors; where the head is less than that, 2^-20 of the largest weight, the rest stays as it is,
+ * since so much for each of many keys would add up. (hi 2^-16 is 0 below 2^-9.) */
+__device__ __forceinline__ uint32_t weight_rest(uint32_t hi, uint32_t rest) {
+    const __half2 s = __half2(__ushort_as_half(0x0100), __ushort_as_half(0x0100)), least = __half2(__ushort_as_half(1), __ushort_as_half(1));
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&rest), __hmin2(__hmul2(*reinterpret_cast<const __half2*>(&hi), s), least));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 /* Two outputs, and the log-sum-exp, from a head's sums (maximum and sum are those of weights times 2^12).
@@ -829,7 +860,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
                         }
                         const uint32_t hi = pack2_rz(w[0], w[1]);
                         const float2 h = unpack2(hi);
-                        const uint32_t lo = hmax2_bits(pack2(w[0] - h.x, w[1] - h.y), 0x00010001u);      /* at least 2^-24 */
+                        const uint32_t lo = weight_rest(hi, pack2(w[0] - h.x, w[1] - h.y));
                         bh[nt][r] = movmatrix(hi);
                         bl[nt][r] = movmatrix(lo);
                     }
