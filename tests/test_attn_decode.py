@@ -234,6 +234,34 @@ def test_attn_nothing_but_empty_sequences(vv):
 
 
 @gpu
+def test_attn_as_many_sequences_as_a_call_takes(vv):
+    lens = np.arange(8192) % 4
+    c = Case(vv, lens, 2, 1, 64, FP16, seed=30).upload()
+    c.check(*c.run())
+    c = Case(vv, np.where(np.arange(8192) == 5000, 700, lens), 1, 1, 64, E4M3, seed=31).upload()
+    c.check(*c.run())
+
+
+@gpu
+def test_attn_cut_work_captured_in_a_graph(vv):
+    """Many items, cut between CTAs: an ordinary launch followed by a dependent one, replayed behind other kernels."""
+    c = Case(vv, [1100, 5, 0, 3000] * 5, 28, 4, 128, E4M3, seed=32, poison=False).upload()
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    src = c.dq.clone()
+    with torch.cuda.graph(g, stream=s):
+        c.dq.copy_(src)
+        for _ in range(3):
+            assert vv.vvb_attn_decode_dev(c.args, s) == 0
+    for lens in (c.lens, c.lens // 2, c.lens):
+        c.dlens.copy_(torch.from_numpy(lens.astype(np.int32)))
+        c.dq.zero_(), c.dout.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        c.lens = lens
+        c.check(c.dout.cpu().numpy(), c.dlse.cpu().numpy())
+
+
+@gpu
 def test_attn_contiguous_cache_shorter_than_its_sequences_claim(vv):
     """Lengths beyond the rows that the cache has: cut there, nothing beyond is read."""
     c = Case(vv, [300, 200], 4, 2, 128, FP16, paged=False, seed=21, slack=0).upload()

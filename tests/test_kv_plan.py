@@ -195,3 +195,26 @@ def test_plan_replayed_from_a_graph_follows_the_lengths(vv):
         lens, table, free = np.array(want["lens"]), want["table"], want["pushed"][: want["count"]]
         if step == 4:
             assert want["status"][5] == 2             # 190 + 2 positions fill its three pages
+
+
+@gpu
+def test_plan_cluster_replayed_from_a_graph(vv):
+    """The forms for long row lists (8 and 16 CTAs), captured and replayed with other lengths."""
+    rng = np.random.default_rng(8)
+    for n, stride, max_rows in ((300, 40, 20000), (900, 40, 80000)):
+        new, lens, table, stack, count, n_pages = build(rng, n, stride, "rows", max_rows)
+        d = Device(new, lens, table, stack, count, n_pages, max_rows)
+        keep = [t.clone() for t in (d.new, d.lens, d.table, d.stack, d.count)]
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        a = d.args(vv)
+        with torch.cuda.graph(g, stream=s):
+            assert vv.vvb_kv_plan_dev(a, s) == 0
+        for change in (np.zeros(n, np.int64), rng.integers(-2, 3, n)):
+            for t, k in zip((d.new, d.lens, d.table, d.stack, d.count), keep):
+                t.copy_(k)
+            tokens = np.where(change < -1, -1, np.maximum(new - np.maximum(change, 0), 0))
+            d.new.copy_(ints(tokens))
+            want = _paged.plan(tokens, lens, table, stack, count, max_rows)
+            g.replay()
+            torch.cuda.synchronize()
+            d.compare(want)

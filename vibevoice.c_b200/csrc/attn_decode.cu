@@ -103,7 +103,7 @@ struct AttnArgs {
     int n_seqs, n_q, n_kv, n_slots, table_stride, len_add;
     int group, head_blocks;    /* query heads to a cache head, items a cache head is cut into */
     int parts;                 /* CTAs of the launch */
-    int by_item, whole_items;
+    int by_item, whole_items, one_each;
     float scale2;              /* scale * log2(e) */
 };
 
@@ -509,53 +509,66 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
      * itself, a lane for every 32nd of the sequences. */
     const int items = A.n_kv * A.head_blocks;
     const bool whole_items = SOLO || A.whole_items;    /* an item belongs to the part in which it begins */
-    const int per = (A.n_seqs + 31) / 32;
-    const int s0 = min(lane * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
-    long long mine = 0;
-#pragma unroll 4
-    for (int b = s0; b < s1; b++) mine += attn_places<BLOCK>(attn_keys(A, b));
-    long long upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-    }
-    const long long total = __shfl_sync(0xffffffffu, upto, 31) * items, before = (upto - mine) * items;
     const int part = SOLO ? blockIdx.x * W + warp : blockIdx.x;
-    /* as few parts as make the largest no larger: 908 places on 444 CTAs are 303 parts of three, not 444 of two or three */
-    const unsigned most = SOLO ? gridDim.x * W : gridDim.x;
-    const long long largest = max(total <= 0x7fffffffll ? (long long)(((unsigned)total + most - 1) / most) : (total + most - 1) / most, 1ll + kAttnItemCost);
-    const int parts = (int)max(total <= 0x7fffffffll ? (long long)(((unsigned)total + (unsigned)largest - 1) / (unsigned)largest) : (total + largest - 1) / largest, 1ll);
-    const AttnCut cut(total, parts);
-    const long long u0 = part < parts ? cut.at(part) : total, u1 = part < parts ? cut.at(part + 1) : total;
-
     AttnAt<BLOCK> to, at;                              /* what is copied next, what is computed next */
-    int places = (int)(u1 - u0), skipped = 0;          /* of the line that are left to this part */
-    if (places > 0) {
-        const int who = __ffs(__ballot_sync(0xffffffffu, u0 >= before && u0 < before + mine * items)) - 1;
-        int b = 0;
-        long long in = 0;                              /* place in sequence b's stretch of the line */
-        if (lane == who) {
-            in = u0 - before;
-            for (b = s0; b < s1; b++) {
-                const long long stretch = (long long)attn_places<BLOCK>(attn_keys(A, b)) * items;
-                if (in < stretch) break;
-                in -= stretch;
+    int places = 0, skipped = 0;                       /* of the line that are left to this part; ahead of its first block */
+    long long u0 = 0, total = 1;
+    AttnCut cut(1, 1);
+    if (A.one_each) {                                  /* fewer items than CTAs, whole: item number `part` */
+        const int b = part / items;
+        if (b < A.n_seqs) {
+            to.set(A, b, part - b * items, 0);
+            places = to.nb;
+        }
+    } else {
+        const int per = (A.n_seqs + 31) / 32;
+        const int s0 = min(lane * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
+        long long mine = 0;
+#pragma unroll 4
+        for (int b = s0; b < s1; b++) mine += attn_places<BLOCK>(attn_keys(A, b));
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        total = __shfl_sync(0xffffffffu, upto, 31) * items;
+        const long long before = (upto - mine) * items;
+        /* as few parts as make the largest no larger: 908 places on 444 CTAs are 303 parts of three, not 444 of two or three */
+        const unsigned most = SOLO ? gridDim.x * W : gridDim.x;
+        const long long largest = max(total <= 0x7fffffffll ? (long long)(((unsigned)total + most - 1) / most) : (total + most - 1) / most, 1ll + kAttnItemCost);
+        const int parts = (int)max(total <= 0x7fffffffll ? (long long)(((unsigned)total + (unsigned)largest - 1) / (unsigned)largest) : (total + largest - 1) / largest, 1ll);
+        cut = AttnCut(total, parts);
+        u0 = part < parts ? cut.at(part) : total;
+        const long long u1 = part < parts ? cut.at(part + 1) : total;
+
+        places = (int)(u1 - u0);
+        if (places > 0) {
+            const int who = __ffs(__ballot_sync(0xffffffffu, u0 >= before && u0 < before + mine * items)) - 1;
+            int b = 0;
+            long long in = 0;                              /* place in sequence b's stretch of the line */
+            if (lane == who) {
+                in = u0 - before;
+                for (b = s0; b < s1; b++) {
+                    const long long stretch = (long long)attn_places<BLOCK>(attn_keys(A, b)) * items;
+                    if (in < stretch) break;
+                    in -= stretch;
+                }
             }
+            b = __shfl_sync(0xffffffffu, b, who);
+            in = __shfl_sync(0xffffffffu, in, who);
+            const int np = attn_places<BLOCK>(attn_keys(A, b));
+            const int item = in <= 0xffffffffll ? (int)((unsigned)in / (unsigned)np) : (int)(in / np);
+            const int off = (int)(in - (long long)item * np);
+            to.set(A, b, item, max(off - kAttnItemCost, 0));
+            skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
+            if (whole_items && off > 0) {                  /* begun in an earlier part */
+                skipped = np - off + kAttnItemCost;
+                if (places > np - off) to.next_item(A, items);
+            }
+            places -= skipped;
+            if (whole_items) places = places + kAttnItemCost > 0 ? max(places, 1) : 0;
         }
-        b = __shfl_sync(0xffffffffu, b, who);
-        in = __shfl_sync(0xffffffffu, in, who);
-        const int np = attn_places<BLOCK>(attn_keys(A, b));
-        const int item = in <= 0xffffffffll ? (int)((unsigned)in / (unsigned)np) : (int)(in / np);
-        const int off = (int)(in - (long long)item * np);
-        to.set(A, b, item, max(off - kAttnItemCost, 0));
-        skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
-        if (whole_items && off > 0) {                  /* begun in an earlier part */
-            skipped = np - off + kAttnItemCost;
-            if (places > np - off) to.next_item(A, items);
-        }
-        places -= skipped;
-        if (whole_items) places = places + kAttnItemCost > 0 ? max(places, 1) : 0;
     }
     /* rows without keys */
     for (int b = blockIdx.x; b < A.n_seqs; b += gridDim.x) {
@@ -710,7 +723,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         int2 d = make_int2(-1, 0);
         if (!began && places >= at.nb - at.blk) {
             const long long first = u0 + skipped - at.blk;       /* place of the item's first block */
-            int p = min((int)((float)first / (float)total * (float)parts), part);
+            int p = min((int)((float)first / (float)total * (float)cut.parts), part);
             while (cut.at(p) > first) p--;
             while (cut.at(p + 1) <= first) p++;
             d = make_int2(A.by_item ? part : at.b * items + at.h, p);
@@ -1087,6 +1100,9 @@ static cudaError_t launch_attn(AttnArgs A, cudaStream_t s) {
     constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM, parts = AttnShape<FMT, HD, NT>::CTAS * kAttnSms;
     static_assert(parts <= kAttnParts, "the scratch holds kAttnParts parts");
     A.parts = parts;
+    const long long items = (long long)A.n_seqs * A.n_kv * A.head_blocks;
+    A.one_each = A.whole_items == 1 && items <= parts;
+    const int ctas = A.one_each ? (int)items : parts;
     const bool solo = A.whole_items == 2;
     cudaError_t e = cudaFuncSetAttribute(solo ? (const void*)attn_decode_kernel<FMT, HD, NT, true> : (const void*)attn_decode_kernel<FMT, HD, NT, false>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
@@ -1096,11 +1112,11 @@ static cudaError_t launch_attn(AttnArgs A, cudaStream_t s) {
      * small CTAs), so this is an ordinary launch unless there are few items: then the launch itself is what counts. */
     const dim3 block(32 * AttnFmt<FMT, HD>::W);
     if (solo) {
-        e = launch_pdl(attn_decode_kernel<FMT, HD, NT, true>, dim3(parts), block, (size_t)SMEM, s, A);
+        e = launch_pdl(attn_decode_kernel<FMT, HD, NT, true>, dim3(ctas), block, (size_t)SMEM, s, A);
     } else if (A.by_item || A.whole_items) {
-        e = launch_pdl(attn_decode_kernel<FMT, HD, NT, false>, dim3(parts), block, (size_t)SMEM, s, A);
+        e = launch_pdl(attn_decode_kernel<FMT, HD, NT, false>, dim3(ctas), block, (size_t)SMEM, s, A);
     } else {
-        attn_decode_kernel<FMT, HD, NT, false><<<dim3(parts), block, (size_t)SMEM, s>>>(A);
+        attn_decode_kernel<FMT, HD, NT, false><<<dim3(ctas), block, (size_t)SMEM, s>>>(A);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) return e;
@@ -1151,7 +1167,7 @@ extern "C" int vvbk_attn_decode(const void* q, void* out, float* lse, const void
                         (const __half*)k_meta, (const __half*)v_meta, block_table, lens,
                         (int2*)base, (float2*)(base + sc.ml), (float4*)(base + sc.o),
                         n_seqs, n_q_heads, n_kv_heads, n_slots, table_stride, len_add,
-                        group, head_blocks, 0, items <= kAttnFewItems, whole, scale * kLog2e};
+                        group, head_blocks, 0, items <= kAttnFewItems, whole, 0, scale * kLog2e};
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
     switch (kv_format) {
