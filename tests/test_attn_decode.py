@@ -203,21 +203,24 @@ def test_attn_long_and_many(vv, lens, fmt, paged):
     c.check(*c.run())
 
 
-# by the positions a table has room for and the number of sequences the work is cut differently: whole sequences to
-# warps or to CTAs, or cut between CTAs with their pieces found by item or by CTA
-WAYS = {"warps": (250, 250, 64), "warps_edge": (222, 256, 0), "ctas": (100, 500, 0), "ctas_few": (2, 190, 64), "ctas_many": (97, 1000, 0),
-        "cut_few": (5, 900, 64), "cut_nine": (9, 2500, 0), "cut": (20, 3000, 64), "cut_many": (300, 1100, 0)}
+# by the blocks a table has room for and the number of sequences the work is cut differently: whole sequences to
+# warps or to CTAs, or cut between CTAs with their pieces found by item or by CTA: sequences, blocks, blocks of the
+# rotated formats
+BLOCK = {FP16: 64, E4M3: 128, E5M2: 128, TQ4: 384, TQ3: 256, TQ2: 256, TQ1_5: 256}
+WAYS = {"warps": (250, 1, 1), "warps_edge": (222, 3, 2), "warps_many": (445, 5, 2), "ctas_few": (2, 8, 4), "ctas": (30, 10, 5), "ctas_many": (150, 4, 4),
+        "ctas_most": (97, 16, 8), "cut_few": (5, 9, 5), "cut_nine": (9, 39, 7), "cut": (20, 12, 6), "cut_many": (112, 17, 9)}
 
 
 @gpu
 @pytest.mark.parametrize("fmt", range(7))
 @pytest.mark.parametrize("way", WAYS)
 def test_attn_every_way_of_cutting_the_work(vv, way, fmt):
-    n, top, room = WAYS[way]
+    n, top = WAYS[way][0], WAYS[way][2 if fmt >= TQ4 else 1] * BLOCK[fmt]
+    top -= n % 7
     rng = np.random.default_rng(n + fmt)
     lens = np.where(rng.random(n) < 0.1, 0, np.exp(rng.uniform(0, np.log(top + 1), n))).astype(np.int64)
     lens[rng.integers(n)] = top
-    c = Case(vv, lens, 16, 4, 128, fmt, seed=n, slack=room // 64).upload()
+    c = Case(vv, lens, 16, 4, 128, fmt, seed=n, slack=0).upload()
     n0 = vv.launch_count()
     out, lse = c.run()
     assert vv.launch_count() - n0 == (2 if way.startswith("cut") else 1)
@@ -240,6 +243,25 @@ def test_attn_as_many_sequences_as_a_call_takes(vv):
     c.check(*c.run())
     c = Case(vv, np.where(np.arange(8192) == 5000, 700, lens), 1, 1, 64, E4M3, seed=31).upload()
     c.check(*c.run())
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[0], [1, 0, 63, 64, 65, 128, 5, 700], [20000, 3, 0, 9000], [40] * 30 + [0, 2000] + [16] * 70])
+def test_attn_tables_for_more_than_32_bits_of_cut_line(vv, lens):
+    """Tables wide enough that the line of blocks, were they full, passes what is cut in 32 bits: the same parts."""
+    width = -(-(1 << 25) // (4 * len(lens)) // 64)      # over 2^21 groups of 16 keys
+    c = Case(vv, lens, 28, 4, 128, FP16, seed=33)
+    wide = np.full((len(lens), max(width, c.table.shape[1])), -1, np.int32)
+    wide[:, :c.table.shape[1]] = c.table
+    outs = []
+    for table in (c.table, wide):
+        c.table, c.stride = table, table.shape[1]
+        c.upload()
+        o, l = c.run()
+        c.check(o, l)
+        outs.append((o, l))
+    if max(lens) > 700:                                 # both are cut, into the same parts
+        assert np.array_equal(outs[0][0].view(np.uint16), outs[1][0].view(np.uint16)) and np.array_equal(outs[0][1], outs[1][1])
 
 
 @gpu

@@ -30,7 +30,7 @@
  * value and needs one byte permute. TurboQuant: two codes index a table in
  * shared memory of two FP16 levels, a copy for each lane, so that 32 lanes never
  * meet in a bank. 16 keys of the 4-bit format are 406 instructions a warp, 70 of
- * them such look-ups (FP16: about 220): it is issue-bound, its ALU pipe first
+ * them such look-ups (FP16: 296, no look-ups): it is issue-bound, its ALU pipe first
  * (tried: entries 128 bytes apart, three CTAs of four warps with a table each:
  * 61.6 us for 48 sequences of 4100 - 8200; 256 apart, where one byte permute
  * forms the address, and twelve warps over one table: 58.9; fourteen and sixteen
@@ -42,7 +42,7 @@
  * inputs give the same bits. The CTA's warps share each block. An item that a
  * CTA holds whole is finished by it, the warps' outputs exchanged in the ring's
  * stage read last; of one that is cut, each CTA leaves its part (running maximum,
- * sum, output) in scratch and a second kernel joins them. attn_way says when
+ * sum, output) in scratch and a second kernel joins them. attn_whole says when
  * items stay whole instead and the second kernel is saved.
  *
  * Measured (28 heads over 4, 128 wide; GB/s of K and V): 64 x 4096 FP16 85.8 us
@@ -81,6 +81,7 @@ constexpr int kAttnPageShift = 6;
 constexpr int kAttnSms = 148, kAttnParts = 3 * kAttnSms;      /* parts the work is cut into, at most */
 constexpr int kAttnFewItems = 37;               /* so many items, in eight tiles each, are one wave of the joining kernel */
 constexpr int kAttnJoinParts = 4, kAttnJoinChunk = 4;
+constexpr int kAttnNarrow = 1 << 22;
 constexpr int kAttnItemCost = 1;                /* what beginning and ending an item costs, in blocks */
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kWeightLog2 = 12.0f;            /* a weight of 1 is kept as 2^12 ... */
@@ -104,6 +105,7 @@ struct AttnArgs {
     int group, head_blocks;    /* query heads to a cache head, items a cache head is cut into */
     int parts;                 /* CTAs of the launch */
     int by_item, whole_items, one_each;
+    int narrow;                /* the line has fewer than kAttnNarrow places */
     float scale2;              /* scale * log2(e) */
 };
 
@@ -473,16 +475,15 @@ template <int BLOCK> struct AttnAt {
     }
 };
 
-/* The line of `total` places cut into `parts` equal parts: place where part p begins, floor(total p / parts). */
-struct AttnCut {
-    long long each;
-    unsigned rest, parts;
-    __device__ __forceinline__ AttnCut(long long total, int n) : parts((unsigned)n) {
-        each = total <= 0xffffffffll ? (long long)((unsigned)total / (unsigned)n) : total / n;
-        rest = (unsigned)(total - each * n);
-    }
-    __device__ __forceinline__ long long at(unsigned p) const { return each * p + rest * p / parts; }
-};
+/* floor(a / b) for 0 <= a < kAttnNarrow, 0 < b <= kAttnNarrow. Both are exact as floats and the quotient is off by
+ * 2 units in the last place, 2^-22 of less than 2^22: its floor is one off at most. */
+__device__ __forceinline__ int attn_div(int a, int b) {
+    int q = (int)__fdividef((float)a, (float)b);
+    q -= q * b > a;
+    q += (q + 1) * b <= a;
+    return q;
+}
+__device__ __forceinline__ long long attn_div(long long a, long long b) { return a / b; }
 
 template <int FMT, int HD, int NT, bool SOLO>
 __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, NT>::CTAS) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
@@ -512,8 +513,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     const int part = SOLO ? blockIdx.x * W + warp : blockIdx.x;
     AttnAt<BLOCK> to, at;                              /* what is copied next, what is computed next */
     int places = 0, skipped = 0;                       /* of the line that are left to this part; ahead of its first block */
-    long long u0 = 0, total = 1;
-    AttnCut cut(1, 1);
+    long long u0 = 0, largest = 1;                     /* the part's first place, and how many a part has */
     if (A.one_each) {                                  /* fewer items than CTAs, whole: item number `part` */
         const int b = part / items;
         if (b < A.n_seqs) {
@@ -521,36 +521,35 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
             places = to.nb;
         }
     } else {
-        const int per = (A.n_seqs + 31) / 32;
-        const int s0 = min(lane * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
-        long long mine = 0;
+        auto find = [&](auto zero) {                   /* in 32-bit numbers where they do: it is 0.8 us before the first load */
+            using T = decltype(zero);
+            const int per = (A.n_seqs + 31) / 32, s0 = min(lane * per, A.n_seqs), s1 = min(s0 + per, A.n_seqs);
+            T mine = 0;
 #pragma unroll 4
-        for (int b = s0; b < s1; b++) mine += attn_places<BLOCK>(attn_keys(A, b));
-        long long upto = mine;
+            for (int b = s0; b < s1; b++) mine += attn_places<BLOCK>(attn_keys(A, b));
+            T upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
-        }
-        total = __shfl_sync(0xffffffffu, upto, 31) * items;
-        const long long before = (upto - mine) * items;
-        /* as few parts as make the largest no larger: 908 places on 444 CTAs are 303 parts of three, not 444 of two or three */
-        const unsigned most = SOLO ? gridDim.x * W : gridDim.x;
-        const long long largest = max(total <= 0x7fffffffll ? (long long)(((unsigned)total + most - 1) / most) : (total + most - 1) / most, 1ll + kAttnItemCost);
-        const int parts = (int)max(total <= 0x7fffffffll ? (long long)(((unsigned)total + (unsigned)largest - 1) / (unsigned)largest) : (total + largest - 1) / largest, 1ll);
-        cut = AttnCut(total, parts);
-        u0 = part < parts ? cut.at(part) : total;
-        const long long u1 = part < parts ? cut.at(part + 1) : total;
-
-        places = (int)(u1 - u0);
-        if (places > 0) {
-            const int who = __ffs(__ballot_sync(0xffffffffu, u0 >= before && u0 < before + mine * items)) - 1;
+            for (int o = 1; o < 32; o <<= 1) {
+                const T x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const T total = __shfl_sync(0xffffffffu, upto, 31) * items, before = (upto - mine) * items;
+            if (total == 0) return;
+            /* as few parts as make the largest no larger: 908 places on 444 CTAs are 303 parts of three, not 444 of two or three */
+            const T most = SOLO ? gridDim.x * W : gridDim.x;
+            const T each = max(attn_div(total + most - 1, most), (T)(1 + kAttnItemCost));
+            const T first = min((T)part * each, total), end = min(first + each, total);
+            u0 = first;
+            largest = each;
+            places = (int)(end - first);
+            if (places <= 0) return;
+            const int who = __ffs(__ballot_sync(0xffffffffu, first >= before && first < before + mine * items)) - 1;
             int b = 0;
-            long long in = 0;                              /* place in sequence b's stretch of the line */
+            T in = 0;                                  /* place in sequence b's stretch of the line */
             if (lane == who) {
-                in = u0 - before;
+                in = first - before;
                 for (b = s0; b < s1; b++) {
-                    const long long stretch = (long long)attn_places<BLOCK>(attn_keys(A, b)) * items;
+                    const T stretch = (T)attn_places<BLOCK>(attn_keys(A, b)) * items;
                     if (in < stretch) break;
                     in -= stretch;
                 }
@@ -558,17 +557,18 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
             b = __shfl_sync(0xffffffffu, b, who);
             in = __shfl_sync(0xffffffffu, in, who);
             const int np = attn_places<BLOCK>(attn_keys(A, b));
-            const int item = in <= 0xffffffffll ? (int)((unsigned)in / (unsigned)np) : (int)(in / np);
-            const int off = (int)(in - (long long)item * np);
+            const int item = (int)attn_div(in, (T)np), off = (int)(in - (T)item * np);
             to.set(A, b, item, max(off - kAttnItemCost, 0));
-            skipped = max(kAttnItemCost - off, 0);         /* the places ahead of the item's first block */
-            if (whole_items && off > 0) {                  /* begun in an earlier part */
+            skipped = max(kAttnItemCost - off, 0);     /* the places ahead of the item's first block */
+            if (whole_items && off > 0) {              /* begun in an earlier part */
                 skipped = np - off + kAttnItemCost;
                 if (places > np - off) to.next_item(A, items);
             }
             places -= skipped;
             if (whole_items) places = places + kAttnItemCost > 0 ? max(places, 1) : 0;
-        }
+        };
+        if (A.narrow) find(0);
+        else find(0ll);
     }
     /* rows without keys */
     for (int b = blockIdx.x; b < A.n_seqs; b += gridDim.x) {
@@ -723,9 +723,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         int2 d = make_int2(-1, 0);
         if (!began && places >= at.nb - at.blk) {
             const long long first = u0 + skipped - at.blk;       /* place of the item's first block */
-            int p = min((int)((float)first / (float)total * (float)cut.parts), part);
-            while (cut.at(p) > first) p--;
-            while (cut.at(p + 1) <= first) p++;
+            const int p = (int)(A.narrow ? (unsigned)first / (unsigned)largest : first / largest);
             d = make_int2(A.by_item ? part : at.b * items + at.h, p);
         }
         if (!A.by_item) A.desc[part] = d;
@@ -1074,15 +1072,25 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
 static int attn_col_tiles(int group, int head_dim, int fmt) { return group > 8 && head_dim <= 128 && fmt != KV_TQ4 ? 2 : 1; }
 
 /* Whether items stay whole, which saves the joining kernel: 2, each a warp's; 1, each a CTA's; 0, they are cut. By
- * the positions that a sequence can have, since its length is known on the device alone. Measured with every
- * sequence as long as that, 28 heads over 4 of 128 in FP16, us (cut / CTA / warp):
- *   1 sequence     64: 5.4 / 4.5 / 5.6    200: 6.9 / 6.5 / 11.0    500: 7.3 / 9.2 / 22.5
- *   32            200: 9.6 / 7.3 / 12.5   500: 13.3 / 13.0 / 28.5  1000: 20.1 / 20.9 / 54.3
- *   96             64: 8.4 / 6.4 / 6.6    500: 25.5 / 20.1 / 33.4  1000: 39.7 / 34.3 / 60.4
- *   300            64: 18.7 / 16.7 / 12.9 200: 31.7 / 27.5 / 26.1  1000: 102 / 96.8 / 96.8 */
-static int attn_whole(long long items, long long capacity) {
-    if (items >= 888 && capacity <= 256) return 2;
-    return capacity <= 256 || (items > 128 && capacity <= 512) || (items >= 384 && capacity <= 1024) ? 1 : 0;
+ * the blocks that a table has room for, since the lengths are known on the device alone: at the limits the best way
+ * loses a little where every sequence fills its table and gains where they do not. The rotated formats take longer
+ * for a block, heads of 256 fill fewer CTAs an SM. Measured, us (cut / CTA / warp), every sequence that long or, the
+ * second triple, from one position to that evenly by the logarithm; 28 heads over 4 of 128:
+ *   items  blocks  FP16                                     4 bits
+ *   4      4       6.7 / 5.3                                12.0 / 13.2 (2: 10.9 / 8.1)
+ *   4      8       7.0 / 7.8 (6: 6.7 / 6.6)                 12.3 / 21.1
+ *   64     4       8.0 / 5.6                                15.8 / 13.5
+ *   64     8       9.4 / 8.4                                18.1 / 21.7
+ *   384    8       25.6 / 19.2        12.0 / 9.0            65.2 / 64.1        24.9 / 30.5
+ *   384    16      39.8 / 33.1        12.9 / 15.9           109 / 114          31.8 / 39.9
+ *   1200   2       22.8 / 20.6 / 18.9 16.5 / 13.7 / 11.8    71.3 / 69.6 / 51.7 48.2 / 43.0 / 35.0
+ *   1200   4       35.6 / 30.6 / 30.3 19.3 / 17.2 / 18.2    104 / 106 / 94.6   51.5 / 50.6 / 72.8
+ *   2400   5             68.7 / 70.2        29.5 / 27.8           227 / 218          92.8 / 115
+ * FP8 and heads of 64 are near FP16's; heads of 256, 384 items, 8 blocks: 48.3 / 53.0, 23.8 / 22.7. */
+static int attn_whole(long long items, long long blocks, bool slow) {
+    if ((items >= 888 && blocks <= (slow ? 2 : 3)) || (items >= 1776 && blocks <= 5 && !slow)) return 2;
+    const int most = items < 64 ? 8 : items < 384 ? 10 : 16;
+    return blocks <= (slow ? most / 2 : most) ? 1 : 0;
 }
 
 struct AttnScratch { size_t ml, o, bytes; };
@@ -1096,11 +1104,12 @@ static AttnScratch attn_scratch(int group, int head_dim) {
 }
 
 template <int FMT, int HD, int NT>
-static cudaError_t launch_attn(AttnArgs A, cudaStream_t s) {
+static cudaError_t launch_attn(AttnArgs A, long long capacity, cudaStream_t s) {
     constexpr int SMEM = AttnShape<FMT, HD, NT>::SMEM, parts = AttnShape<FMT, HD, NT>::CTAS * kAttnSms;
     static_assert(parts <= kAttnParts, "the scratch holds kAttnParts parts");
     A.parts = parts;
     const long long items = (long long)A.n_seqs * A.n_kv * A.head_blocks;
+    A.whole_items = attn_whole(items, (capacity + AttnFmt<FMT, HD>::BLOCK - 1) / AttnFmt<FMT, HD>::BLOCK, kv_is_tq(FMT) || HD == 256);
     A.one_each = A.whole_items == 1 && items <= parts;
     const int ctas = A.one_each ? (int)items : parts;
     const bool solo = A.whole_items == 2;
@@ -1129,16 +1138,16 @@ static cudaError_t launch_attn(AttnArgs A, cudaStream_t s) {
     return e;
 }
 template <int FMT>
-static cudaError_t launch_attn(const AttnArgs& A, int head_dim, int nt, cudaStream_t s) {
+static cudaError_t launch_attn(const AttnArgs& A, int head_dim, int nt, long long capacity, cudaStream_t s) {
     if constexpr (!kv_is_tq(FMT)) {
-        if (head_dim == 64) return nt == 2 ? launch_attn<FMT, 64, 2>(A, s) : launch_attn<FMT, 64, 1>(A, s);
-        if (head_dim == 256) return launch_attn<FMT, 256, 1>(A, s);
+        if (head_dim == 64) return nt == 2 ? launch_attn<FMT, 64, 2>(A, capacity, s) : launch_attn<FMT, 64, 1>(A, capacity, s);
+        if (head_dim == 256) return launch_attn<FMT, 256, 1>(A, capacity, s);
     }
     if (head_dim == 128) {
         if constexpr (FMT != KV_TQ4) {
-            if (nt == 2) return launch_attn<FMT, 128, 2>(A, s);
+            if (nt == 2) return launch_attn<FMT, 128, 2>(A, capacity, s);
         }
-        return launch_attn<FMT, 128, 1>(A, s);
+        return launch_attn<FMT, 128, 1>(A, capacity, s);
     }
     return cudaErrorNotSupported;
 }
@@ -1162,22 +1171,21 @@ extern "C" int vvbk_attn_decode(const void* q, void* out, float* lse, const void
     const int head_blocks = (group + 8 * nt - 1) / (8 * nt);
     const long long items = (long long)n_seqs * n_kv_heads * head_blocks;
     const long long capacity = block_table != nullptr ? (long long)table_stride << kAttnPageShift : (long long)table_stride;
-    const int whole = attn_whole(items, capacity);
     const AttnArgs A = {(const __half*)q, (__half*)out, lse, (const uint8_t*)k_store, (const uint8_t*)v_store,
                         (const __half*)k_meta, (const __half*)v_meta, block_table, lens,
                         (int2*)base, (float2*)(base + sc.ml), (float4*)(base + sc.o),
                         n_seqs, n_q_heads, n_kv_heads, n_slots, table_stride, len_add,
-                        group, head_blocks, 0, items <= kAttnFewItems, whole, 0, scale * kLog2e};
+                        group, head_blocks, 0, items <= kAttnFewItems, 0, 0, items * (capacity / 16 + 2) < kAttnNarrow / 2, scale * kLog2e};
     cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
     switch (kv_format) {
-        case KV_RAW: e = launch_attn<KV_RAW>(A, head_dim, nt, s); break;
-        case KV_E4M3: e = launch_attn<KV_E4M3>(A, head_dim, nt, s); break;
-        case KV_E5M2: e = launch_attn<KV_E5M2>(A, head_dim, nt, s); break;
-        case KV_TQ4: e = launch_attn<KV_TQ4>(A, head_dim, nt, s); break;
-        case KV_TQ3: e = launch_attn<KV_TQ3>(A, head_dim, nt, s); break;
-        case KV_TQ2: e = launch_attn<KV_TQ2>(A, head_dim, nt, s); break;
-        case KV_TQ1_5: e = launch_attn<KV_TQ1_5>(A, head_dim, nt, s); break;
+        case KV_RAW: e = launch_attn<KV_RAW>(A, head_dim, nt, capacity, s); break;
+        case KV_E4M3: e = launch_attn<KV_E4M3>(A, head_dim, nt, capacity, s); break;
+        case KV_E5M2: e = launch_attn<KV_E5M2>(A, head_dim, nt, capacity, s); break;
+        case KV_TQ4: e = launch_attn<KV_TQ4>(A, head_dim, nt, capacity, s); break;
+        case KV_TQ3: e = launch_attn<KV_TQ3>(A, head_dim, nt, capacity, s); break;
+        case KV_TQ2: e = launch_attn<KV_TQ2>(A, head_dim, nt, capacity, s); break;
+        case KV_TQ1_5: e = launch_attn<KV_TQ1_5>(A, head_dim, nt, capacity, s); break;
         default: return (int)cudaErrorNotSupported;
     }
     return (int)(e != cudaSuccess ? e : cudaGetLastError());
