@@ -208,7 +208,7 @@ def test_attn_long_and_many(vv, lens, fmt, paged):
 # rotated formats
 BLOCK = {FP16: 64, E4M3: 128, E5M2: 128, TQ4: 384, TQ3: 256, TQ2: 256, TQ1_5: 256}
 WAYS = {"warps": (250, 1, 1), "warps_edge": (222, 3, 2), "warps_many": (445, 5, 2), "ctas_few": (2, 8, 4), "ctas": (30, 10, 5), "ctas_many": (150, 4, 4),
-        "ctas_most": (97, 16, 8), "cut_few": (5, 9, 5), "cut_nine": (9, 39, 7), "cut": (20, 12, 6), "cut_many": (112, 17, 9)}
+        "ctas_most": (97, 16, 7), "cut_few": (5, 9, 5), "cut_nine": (9, 39, 7), "cut": (20, 12, 6), "cut_many": (112, 17, 9)}
 
 
 @gpu

@@ -1078,10 +1078,10 @@ static int attn_col_tiles(int group, int head_dim, int fmt) { return group > 8 &
  * second triple, from one position to that evenly by the logarithm; 28 heads over 4 of 128:
  *   items  blocks  FP16                                     4 bits
  *   4      4       6.7 / 5.3                                12.0 / 13.2 (2: 10.9 / 8.1)
- *   4      8       7.0 / 7.8 (6: 6.7 / 6.6)                 12.3 / 21.1
+ *   4      8       7.0 / 7.8 (6: 6.7 / 6.6)                 11.9 / 19.0 (7)
  *   64     4       8.0 / 5.6                                15.8 / 13.5
- *   64     8       9.4 / 8.4                                18.1 / 21.7
- *   384    8       25.6 / 19.2        12.0 / 9.0            65.2 / 64.1        24.9 / 30.5
+ *   64     8       9.4 / 8.4                                17.1 / 19.5 (7)
+ *   384    8       25.6 / 19.2        12.0 / 9.0            57.5 / 57.9 (7)    24.5 / 28.4
  *   384    16      39.8 / 33.1        12.9 / 15.9           109 / 114          31.8 / 39.9
  *   1200   2       22.8 / 20.6 / 18.9 16.5 / 13.7 / 11.8    71.3 / 69.6 / 51.7 48.2 / 43.0 / 35.0
  *   1200   4       35.6 / 30.6 / 30.3 19.3 / 17.2 / 18.2    104 / 106 / 94.6   51.5 / 50.6 / 72.8
