@@ -430,7 +430,7 @@ vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* args, void* str
  *  no initialisation; calls that overlap on a GPU need one each (two captured
  *  graphs may share one when they do not run at the same time). The work is
  *  split over the SMs by the lengths read on the device and joined in an order
- *  that the lengths alone decide: the same inputs give the same bits. */
+ *  that lengths and sizes alone decide: the same call gives the same bits. */
 typedef struct vvb_attn_decode {
     const void* q;             /* FP16 [n_seqs, n_q_heads, head_dim] */
     void* out;                 /* FP16 [n_seqs, n_q_heads, head_dim] */

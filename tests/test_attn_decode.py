@@ -265,6 +265,22 @@ def test_attn_tables_for_more_than_32_bits_of_cut_line(vv, lens):
 
 
 @gpu
+@pytest.mark.parametrize("lens", [[900, 0, 5, 70], [0, 0, 64, 9000], [1100, 5, 0, 3000] * 5])
+def test_attn_scratch_of_zeros_or_of_another_call(vv, lens):
+    c = Case(vv, lens, 28, 4, 128, FP16, seed=34).upload()
+    want = c.run()
+    c.check(*want)
+    for other in (None, [3000] * 20, [7000, 3], [0, 40]):
+        c.scratch[:-16].zero_()
+        if other is not None:
+            x = Case(vv, other, 28, 4, 128, FP16, seed=35).upload()
+            x.args.scratch = c.args.scratch
+            x.run()
+        got = c.run()
+        assert np.array_equal(got[0].view(np.uint16), want[0].view(np.uint16)) and np.array_equal(got[1], want[1])
+
+
+@gpu
 def test_attn_cut_work_captured_in_a_graph(vv):
     """Many items, cut between CTAs: an ordinary launch followed by a dependent one, replayed behind other kernels."""
     c = Case(vv, [1100, 5, 0, 3000] * 5, 28, 4, 128, E4M3, seed=32, poison=False).upload()

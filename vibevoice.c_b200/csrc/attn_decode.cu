@@ -39,8 +39,9 @@
  * Work: the blocks of 64 (128, 256, 384) positions of all items in one line, cut
  * into equal parts, one for each CTA that fits the GPU at once. The cut depends
  * on the lengths alone, which every warp sums up on the device, so the same
- * inputs give the same bits. The CTA's warps share each block. An item that a
- * CTA holds whole is finished by it, the warps' outputs exchanged in the ring's
+ * inputs give the same bits. (A line of less than 2^22 places is cut in 32-bit
+ * numbers without a long division ahead of the first load: 0.45 us a call.) The
+ * CTA's warps share each block. An item that a CTA holds whole is finished by it, the warps' outputs exchanged in the ring's
  * stage read last; of one that is cut, each CTA leaves its part (running maximum,
  * sum, output) in scratch and a second kernel joins them. attn_whole says when
  * items stay whole instead and the second kernel is saved.
@@ -48,19 +49,19 @@
  * Measured (28 heads over 4, 128 wide; GB/s of K and V): 64 x 4096 FP16 85.8 us
  * = 6.26 TB/s, 0.95 of the device's copy rate; 96 sequences of 1 .. 16384 57.6 us,
  * 0.85; 48 of 4100 .. 8200 in FP8 53.5 us, 0.85; the same in 4 bits 58.9 us, 0.40;
- * 1 x 14449 FP16 12.6 us, latency: the first loads behind lens and table, three
- * steps, and the join. Bytes in flight: one stage of 8 KB for each of 12 warps an
- * SM beside the one being read; two stages are slower (89.4 us for 64 x 4096),
+ * 1 x 14449 FP16 11.9 us, latency: the first loads behind lens and table, three
+ * steps, and the join; 1 x 300 6.0, 1 x 64 3.5, whole items in one kernel. Bytes in
+ * flight: one stage of 8 KB for each of 12 warps an SM beside the one being read; two stages are slower (89.4 us for 64 x 4096),
  * and so are two CTAs an SM (88.3).
  * A cluster of eight CTAs for an item, joined through distributed shared memory
- * in one launch, costs more than the second kernel (1 x 300: 8.4 us, 7.1).
+ * in one launch, costs more than the second kernel (1 x 300, cut: 8.4 us, 7.1).
  *
  * Precision: scores, maximum, sums and outputs in FP32. A weight e^(s - m), times
  * 2^12, goes to the tensor cores as a pair of FP16 values, the one rounded toward
  * zero and the rest: one FP16 value alone would add an error as large as the
  * output's own rounding. Where a weight matters both are positive (weight_rest), so
- * that an infinity in V stays one; below 2^-37 of the largest it is nothing. The maximum follows the scores only beyond a factor of 2^3 (8 % of
- * the steps instead of 41 % for normal scores over 600 keys): 2^15 is the largest
+ * that an infinity in V stays one; below 2^-37 of the largest it is nothing. The
+ * maximum follows the scores only beyond a factor of 2^3 (8 % of the steps instead of 41 % for normal scores over 600 keys): 2^15 is the largest
  * weight then. For the rotated
  * formats the levels times a common factor become FP16 values within 9e-5 of
  * themselves (attn_alpha, found by trying factors in [1, 2); 1.6e-4 for the
