@@ -298,7 +298,7 @@ def _plan(s):
     have = (lens + PAGE - 1) // PAGE
     start = torch.cat([torch.zeros(1, dtype=torch.long, device=dev), add.cumsum(0)])
     full = ~ends & (lens + add > width * PAGE)
-    no_rows = (add > 0) & ~full & (start[1:] > c["rows"])
+    no_rows = ~ends & ~full & (start[1:] > c["rows"])
     need = torch.where(ends | full | no_rows, 0, (lens + add + PAGE - 1) // PAGE - have)
     # released pages go onto the stack in order
     freed = torch.where(ends, have, 0)
