@@ -107,6 +107,8 @@ __device__ __forceinline__ size_t cache_row(const int* page_table, int t) {
     return ((size_t)__ldg(page_table + (t >> kKvPageShift)) << kKvPageShift) + (size_t)(t & ((1 << kKvPageShift) - 1));
 }
 
+constexpr int kStageVecs = 512;      /* 16-byte pieces of a CTA's rotated K that wait for their encoding */
+
 enum { kAddrFlat = 0, kAddrPaged = 1, kAddrSlots = 2 };
 
 /* Cache row of row r, -1 for none; `first` is the logical position of row 0. */
@@ -266,7 +268,6 @@ rope_append_kernel(const __grid_constant__ RopeAppendArgs A) {
 
     /* FP8: the K columns of this CTA's column chunk are staged through shared
      * memory (phase D) when the tile fits: 4 rows x 4 heads of 128 are 256 vectors. */
-    constexpr int kStageVecs = 512;
     __shared__ vec16 k_stage[FMT == KV_RAW ? 1 : kStageVecs];
     const int chunk0 = by * kRopeThreads;
     const int chunk1 = min(chunk0 + a.cols_per_cta, a.items_per_row);
@@ -517,13 +518,15 @@ extern "C" int vvbk_rope_append(void* q, void* k, const void* v,
     RopeAppendArgs A;
     unsigned gx, gy;
     /* a flat grid: the V CTAs first, then the tiles over the Q and K heads */
-    /* TurboQuant: the CTA's rotated K tile (its K columns x 2 halves x its rows) must fit the
-     * 512-vector staging buffer, which bounds the rows a CTA takes */
+    /* TurboQuant: the CTA's rotated K tile (its K columns x 2 halves x its rows) must fit the staging
+     * buffer, which bounds the rows a CTA takes: row_slots (rope_plan) for each pass. One pass always
+     * fits: kcols <= cols and cols * (kRopeThreads / cols) <= kRopeThreads. */
     int max_passes = kRopeMaxRowsPerThread;
     if (tq) {
-        const int kcols = n_kv_heads * (head_dim / 16);          /* <= 256: one column chunk holds them all */
-        const int fit = 512 / (2 * kcols);
-        if (fit < 1) return (int)cudaErrorNotSupported;
+        static_assert(2 * kRopeThreads <= kStageVecs, "one pass fits the staging buffer");
+        const int kcols = min(n_kv_heads * (head_dim / 16), kRopeThreads);
+        const int cols = min((n_q_heads + n_kv_heads) * (head_dim / 16), kRopeThreads);
+        const int fit = kStageVecs / (2 * kcols * (kRopeThreads / cols));
         if (max_passes > fit) max_passes = fit;
     }
     rope_plan(A.r, q, k, rows, n_q_heads, n_kv_heads, head_dim, position_offset, d_position, inv_freq,
