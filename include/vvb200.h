@@ -413,7 +413,9 @@ vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* args, void* str
  *    s_j = scale * q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),
  *    lse = m + ln sum_j e^(s_j - m),  m = max_j s_j,
  *  every sum, the maximum and the scores in FP32. A sequence without keys (or a
- *  head all of whose scores are -inf) gets zeros and lse = -inf. Key j lies in cache row block_table[b][j / 64] * 64 + j % 64, or with
+ *  head all of whose scores are -inf) gets zeros and lse = -inf. An infinity in V has
+ *  its sign in the result, however small its weight is beside the others'.
+ *  Key j lies in cache row block_table[b][j / 64] * 64 + j % 64, or with
  *  block_table == NULL in row b * table_stride + j (table_stride: rows of the
  *  cache per sequence). n is cut to the 64 * table_stride (table_stride) positions
  *  that there are, and to 0 below it; keys whose row lies outside [0, n_slots)

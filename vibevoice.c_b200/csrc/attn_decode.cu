@@ -59,8 +59,10 @@
  * Precision: scores, maximum, sums and outputs in FP32. A weight e^(s - m), times
  * 2^12, goes to the tensor cores as a pair of FP16 values, the one rounded toward
  * zero and the rest: one FP16 value alone would add an error as large as the
- * output's own rounding. Where a weight matters both are positive (weight_rest), so
- * that an infinity in V stays one; below 2^-37 of the largest it is nothing. The
+ * output's own rounding; below 2^-37 of the largest a weight is nothing. An infinity
+ * in V meets two positive factors where its weight is 2^-20 of the largest or more
+ * (weight_rest); under less it can make the sum a NaN, which is then looked up
+ * (attn_infinite). The
  * maximum follows the scores only beyond a factor of 2^3 (8 % of the steps instead of 41 % for normal scores over 600 keys): 2^15 is the largest
  * weight then. For the rotated
  * formats the levels times a common factor become FP16 values within 9e-5 of
@@ -88,6 +90,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kWeightLog2 = 12.0f;            /* a weight of 1 is kept as 2^12 ... */
 constexpr float kWeightTop = 15.0f;             /* ... and the maximum follows the scores once one passes 2^15 */
 constexpr float kNoMax = -3e38f;
+constexpr unsigned short kAttnMark = 0x7fff;    /* an output to look up (attn_infinite) */
 
 struct AttnArgs {
     const __half* q;
@@ -181,17 +184,21 @@ __device__ __forceinline__ uint32_t pack2_rz(float a, float b) {       /* two ha
 }
 /* The rest of two weights whose heads are `hi`: at least 2^-24 where the head is 2^-8 or more, so that an infinity in V
  * meets two positive factors; where the head is less than that, 2^-20 of the largest weight, the rest stays as it is,
- * since so much for each of many keys would add up. (hi 2^-16 is 0 below 2^-9.) */
+ * since so much for each of many keys would add up (hi 2^-16 is 0 below 2^-9), and attn_infinite has the last word. */
 __device__ __forceinline__ uint32_t weight_rest(uint32_t hi, uint32_t rest) {
     const __half2 s = __half2(__ushort_as_half(0x0100), __ushort_as_half(0x0100)), least = __half2(__ushort_as_half(1), __ushort_as_half(1));
     const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&rest), __hmin2(__hmul2(*reinterpret_cast<const __half2*>(&hi), s), least));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 /* Two outputs, and the log-sum-exp, from a head's sums (maximum and sum are those of weights times 2^12).
- * A sum of zero: no keys, or none with a score above -inf. */
-__device__ __forceinline__ uint32_t attn_out(float a, float b, float sum) {
+ * A sum of zero: no keys, or none with a score above -inf. A sum that is NaN: outputs 0x7e00; any other NaN is what
+ * the conversion makes of it, kAttnMark, and `odd` says that there may be one. */
+__device__ __forceinline__ uint32_t attn_out(float a, float b, float sum, bool& odd) {
     const float r = 1.0f / sum;
-    return sum == 0.0f ? 0u : pack2(a * r, b * r);
+    a *= r;
+    b *= r;
+    if (a != a || b != b) odd = true;
+    return sum == 0.0f ? 0u : sum != sum ? 0x7e007e00u : pack2(a, b);
 }
 __device__ __forceinline__ float attn_lse(float top, float sum) {
     return sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
@@ -476,6 +483,59 @@ template <int BLOCK> struct AttnAt {
     }
 };
 
+/* The sign of the stored value at `dim` of a row of V that holds codes (none of the levels is 0). */
+template <int FMT> __device__ __forceinline__ bool attn_code_negative(const uint8_t* row, int dim) {
+    constexpr int NB = FMT == KV_TQ4 ? 4 : FMT == KV_TQ2 ? 2 : 3;
+    const int bit = NB * (FMT == KV_TQ1_5 ? dim >> 1 : dim);
+    unsigned w = row[bit >> 3];
+    if ((bit & 7) + NB > 8) w |= (unsigned)row[(bit >> 3) + 1] << 8;
+    const unsigned c = (w >> (bit & 7)) & ((1u << NB) - 1u);
+    return FMT == KV_TQ1_5 ? c_vq15[2 * c + (dim & 1)] < 0.0f : c < (1u << (NB - 1));
+}
+/* What a NaN in an output stands for whose scores are no NaN: infinities in V, which have their sign in the result
+ * under any weight of a finite score, but are NaN where the weight, or a half of it, is 0 in FP16 or in FP32. So V
+ * is looked through at that dim, a key at a time: it happens to infinite values only. (Infinities of both signs and
+ * NaNs give NaN. V of a key whose score is -inf counts as any.) */
+template <int FMT, int HD> __device__ float attn_infinite(const AttnArgs& A, int b, int hk, int dim) {
+    constexpr int VEC = AttnFmt<FMT, HD>::VEC;
+    const int n = attn_keys(A, b);
+    bool pos = false, neg = false, nan = false;
+    for (int j = 0; j < n && !nan && !(pos && neg); j++) {
+        long long row = (long long)b * A.table_stride + j;
+        if (A.block_table != nullptr) {
+            const int page = __ldg(A.block_table + (size_t)b * A.table_stride + (j >> kAttnPageShift));
+            if ((unsigned)page > (unsigned)(A.n_slots - 1) >> kAttnPageShift) continue;
+            row = ((long long)page << kAttnPageShift) + (j & 63);
+        }
+        if (row >= A.n_slots) continue;
+        const size_t at = (size_t)row * A.n_kv + hk;
+        if constexpr (kv_is_tq(FMT)) {
+            const float rms = __half2float(A.v_meta[at]);
+            nan |= rms != rms;
+            if (rms == INFINITY) (attn_code_negative<FMT>(A.v_store + at * VEC, dim) ? neg : pos) = true;
+        } else {
+            const float v = FMT == KV_RAW ? __half2float(reinterpret_cast<const __half*>(A.v_store)[at * HD + dim])
+                                          : __half2float(__ushort_as_half((unsigned short)(A.v_store[at * VEC + dim] << 8)));
+            nan |= v != v;
+            pos |= v == INFINITY;
+            neg |= v == -INFINITY;
+        }
+    }
+    return nan || pos == neg ? __int_as_float(0x7fffffff) : pos ? INFINITY : -INFINITY;
+}
+/* Outputs of items first .. last (whole ones, by their places in the line) that attn_out has marked. Called once they
+ * are all written, by `threads` threads, so that what it takes is not paid for where there are none. */
+template <int FMT, int HD> __device__ __noinline__ void attn_look_up(const AttnArgs& A, int first, int last, int heads_of, int thread, int threads) {
+    const int items = A.n_kv * A.head_blocks;
+    for (int i = first; i <= last; i++) {
+        const int b = i / items, h = i - b * items, hk = h / A.head_blocks, h0 = (h - hk * A.head_blocks) * heads_of;
+        if (attn_keys(A, b) == 0) continue;            /* zeros, perhaps another CTA's, and perhaps not written yet */
+        __half* const o = A.out + ((size_t)b * A.n_q + (size_t)hk * A.group + h0) * HD;
+        for (int e = thread; e < min(heads_of, A.group - h0) * HD; e += threads)
+            if (__half_as_ushort(o[e]) == kAttnMark) o[e] = __float2half(attn_infinite<FMT, HD>(A, b, hk, e % HD));
+    }
+}
+
 /* floor(a / b) for 0 <= a < kAttnNarrow, 0 < b <= kAttnNarrow. Both are exact as floats and the quotient is off by
  * 2 units in the last place, 2^-22 of less than 2^22: its floor is one off at most. */
 __device__ __forceinline__ int attn_div(int a, int b) {
@@ -586,6 +646,9 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
     }
     at = to;
     bool began = at.blk == 0;                          /* this part holds the beginning of the item */
+    [[maybe_unused]] __shared__ int first_s[SOLO ? W : 1];       /* the first item that is whole here, for the look-up at the end */
+    if (SOLO ? lane == 0 : tid == 0) first_s[SOLO ? warp : 0] = at.b * items + at.h + (began ? 0 : 1);
+    bool odd = false;
 
     /* What is copied next: units lane, lane + 32, .. of the group's rows. The pointers are those of the first
      * of them in row 0 of the cache. */
@@ -827,8 +890,8 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
                     float x = sv_top;
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    if (x > vref) {                    /* the next power of two above it */
-                        const float nref = x < INFINITY ? __uint_as_float((__float_as_uint(x) & 0x7f800000u) + 0x00800000u) : vref;
+                    if (x > vref) {                    /* the next power of two above it, or above all finite ones */
+                        const float nref = x < INFINITY ? __uint_as_float((__float_as_uint(x) & 0x7f800000u) + 0x00800000u) : 65536.0f;
                         rv = vref / nref;
                         vref = nref;
                     }
@@ -915,7 +978,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
                     const float f = vref * (1.0f / attn_alpha<FMT>());
 #pragma unroll
                     for (int j = 0; j < TILES; j++)
-                        attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(o[nt][j][c] * f, o[nt][j][c + 2] * f, l[nt][c]));
+                        attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(o[nt][j][c] * f, o[nt][j][c + 2] * f, l[nt][c], odd));
                     if (A.lse != nullptr && g == 0) A.lse[head0 + h] = attn_lse(m[nt][c], l[nt][c]);
                 }
         } else {
@@ -974,7 +1037,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const int h = 8 * nt + 2 * t + c;
-                        if (h < heads) attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(acc[c], acc[c + 2], sum[c]));
+                        if (h < heads) attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(acc[c], acc[c + 2], sum[c], odd));
                     }
                 } else {
                     A.part_o[((size_t)slot * (NT * TILES) + x) * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -990,6 +1053,13 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         begin_item();
     }
     cp_wait<0>();
+    if constexpr (FMT != KV_E4M3) {                    /* (it has no infinities) */
+        if (SOLO ? __any_sync(0xffffffffu, odd) : __syncthreads_or(odd)) {
+            const int last = at.b * items + at.h - (SOLO || at.last() ? 0 : 1);
+            if (SOLO) __syncwarp();                    /* (all outputs are written; a barrier does it for the CTA) */
+            attn_look_up<FMT, HD>(A, first_s[SOLO ? warp : 0], last, 8 * NT, SOLO ? lane : tid, SOLO ? 32 : 32 * W);
+        }
+    }
 }
 
 /* Joins the pieces of items that are cut: an item that ends in part `last` and began in part `first` has them in
@@ -1062,8 +1132,19 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
         for (int c = 0; c < 2; c++) {
             const int h = 8 * nt + 2 * t + c;
             if (h >= heads) continue;
-            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(s.o[c], s.o[c + 2], s.l[c]));
+            bool odd = false;
+            const uint32_t two = attn_out(s.o[c], s.o[c + 2], s.l[c], odd);
+            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, two);
             if (A.lse != nullptr && j == 0 && g == 0) A.lse[head0 + h] = attn_lse(s.m[c], s.l[c]);
+            if constexpr (FMT != KV_E4M3) {
+                if (!odd) continue;
+#pragma unroll 1
+                for (int e = 2 * j; e < 2 * j + 2; e++) {
+                    const int dim = attn_v_dim<FMT>(e, g);
+                    __half* const out = A.out + (head0 + h) * HD + dim;
+                    if (__half_as_ushort(*out) == kAttnMark) *out = __float2half(attn_infinite<FMT, HD>(A, b, hk, dim));
+                }
+            }
         }
     }
 }
