@@ -12,7 +12,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("max_rows", [(8192, 3000), (40000, 40000)])
+@pytest.mark.parametrize("max_rows", [(4096, 3000), (40000, 40000)])
 def test_two_threads_plan_different_numbers_of_sequences(max_rows):
     if not torch.cuda.is_available():
         pytest.skip("no CUDA device")

@@ -34,6 +34,8 @@ namespace vvb {
 extern std::atomic<uint64_t> g_launches;
 
 constexpr int kPlanPageShift = 6;
+constexpr int kPlanMaxSeqs = 8192;
+constexpr size_t plan_smem_bytes(int n_seqs) { return (5 * (size_t)n_seqs + 3) * sizeof(int); }      /* 160 KB at most */
 
 struct PlanArgs {
     const int* new_tokens;
@@ -246,10 +248,11 @@ extern "C" int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_ou
      * by opt-in) from where that shows: 131072 rows of 2000 sequences 14.6 us with 8, 11.1 with 16. */
     const int ctas = max_rows > 32768 ? 16 : max_rows > 4096 ? 8 : 1;
     const bool cluster = ctas > 1;
-    const size_t smem = (5 * (size_t)n_seqs + 3) * sizeof(int);       /* n_seqs <= 8192: 160 KB */
+    const size_t smem = plan_smem_bytes(n_seqs);
     void (*kernel)(const PlanArgs) = cluster ? kv_plan_kernel<true> : kv_plan_kernel<false>;
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        /* the most that any call asks for: the attribute is the function's, and another thread may be about to launch */
+        const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem_bytes(kPlanMaxSeqs));
         if (e != cudaSuccess) return (int)e;
     }
     if (ctas > 8) {
