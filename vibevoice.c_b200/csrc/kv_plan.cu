@@ -118,13 +118,14 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
     const unsigned cap = (unsigned)A.table_stride << kPlanPageShift;         /* < 2^31 */
     auto pages_of = [&](int len) { return min(((unsigned)len + 63u) >> kPlanPageShift, (unsigned)A.table_stride); };
     auto full = [&](int add, int len) { return add >= 0 && ((unsigned)len > cap || (unsigned)add > cap - (unsigned)len); };
-    const unsigned held = (unsigned)min(max(__ldg(A.free_count), 0), A.n_pages);
+    /* lens and the height may be overwritten below (lens_out, free_count_out), so they are not read-only data */
+    const unsigned held = (unsigned)min(max(__ldcg(A.free_count), 0), A.n_pages);
     const int per = (n + nt - 1) / nt;
     const int b0 = min(t * per, n), b1 = min(b0 + per, n);
     /* rows and released pages */
     unsigned rows = 0, rel = 0;
     for (int b = b0; b < b1; b++) {
-        const int add = __ldg(A.new_tokens + b), len = max(__ldg(A.lens + b), 0);
+        const int add = __ldg(A.new_tokens + b), len = max(__ldcg(A.lens + b), 0);
         new_s[b] = add;
         base_s[b] = len;
         rows = sat_add(rows, (unsigned)max(add, 0));
