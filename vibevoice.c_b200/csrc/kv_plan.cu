@@ -236,6 +236,34 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
     }
 }
 
+/* Whether the current device has room for a cluster of 16 such CTAs, which a part of a GPU need not have; asked once a
+ * device. The attributes are the same in every call, so threads may come at the same time. */
+static bool plan_wide_clusters() {
+    static std::atomic<signed char> known[64];             /* 0: not asked; 1: no; 2: yes */
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    const signed char k = known[dev].load(std::memory_order_relaxed);
+    if (k != 0) return k == 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = plan_smem_bytes(kPlanMaxSeqs);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 16;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    const void* f = (const void*)kv_plan_kernel<true>;
+    bool ok = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem_bytes(kPlanMaxSeqs)) == cudaSuccess &&
+              cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+              cudaOccupancyMaxActiveClusters(&fit, kv_plan_kernel<true>, &cfg) == cudaSuccess && fit > 0;
+    if (!ok) cudaGetLastError();                           /* eight will do */
+    known[dev].store(ok ? 2 : 1, std::memory_order_relaxed);
+    return ok;
+}
+
 }  // namespace vvb
 
 using namespace vvb;
@@ -246,18 +274,14 @@ extern "C" int vvbk_kv_plan(const int* new_tokens, const int* lens, int* lens_ou
     const PlanArgs A = {new_tokens, lens, lens_out, block_table, free_pages, free_count, free_count_out, row_start,
                         slot_map, positions, status, n_seqs, table_stride, n_pages, max_rows};
     /* Rows are what takes time beyond the first few thousand, 1024 threads a CTA; 16 CTAs (the most a cluster can have,
-     * by opt-in) from where that shows: 131072 rows of 2000 sequences 14.6 us with 8, 11.1 with 16. */
-    const int ctas = max_rows > 32768 ? 16 : max_rows > 4096 ? 8 : 1;
+     * by opt-in) from where that shows and the GPU has room: 131072 rows of 2000 sequences 14.6 us with 8, 11.1 with 16. */
+    const int ctas = max_rows <= 4096 ? 1 : max_rows > 32768 && plan_wide_clusters() ? 16 : 8;
     const bool cluster = ctas > 1;
     const size_t smem = plan_smem_bytes(n_seqs);
     void (*kernel)(const PlanArgs) = cluster ? kv_plan_kernel<true> : kv_plan_kernel<false>;
     if (smem > 48 * 1024) {
         /* the most that any call asks for: the attribute is the function's, and another thread may be about to launch */
         const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem_bytes(kPlanMaxSeqs));
-        if (e != cudaSuccess) return (int)e;
-    }
-    if (ctas > 8) {
-        const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return (int)e;
     }
     cudaLaunchConfig_t cfg = {};
