@@ -354,7 +354,8 @@ vv_status_t vvb_kv_unrotate_dev(void* x_fp16, int n_heads, int head_dim, int row
  *  max_rows. Sequences are admitted in order: one is refused for pages when the
  *  pages asked for up to and including it exceed the stack's height, so a later
  *  sequence is never admitted in an earlier one's place unless it needs none.
- *  A page belongs to one sequence: what two tables name is pushed twice.
+ *  A page belongs to one sequence: what two tables name is pushed twice. Rows on
+ *  what is no page of the pool (an entry outside [0, n_pages)) get slot -1.
  *  lens_out may be lens and free_count_out may be free_count; no other two
  *  arrays may overlap. Table entries beyond a sequence's pages are not touched.
  *  The result does not depend on timing. 1 <= table_stride <= 2^25 - 1, n_pages

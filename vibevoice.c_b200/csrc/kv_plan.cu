@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(1024, 1) kv_plan_kernel(const __grid_constant_
         }
 #pragma unroll
         for (int j = 0; j < kRun; j++)
-            if (pos[j] >= 0) slot[j] = (int)(((unsigned)slot[j] << kPlanPageShift) + ((unsigned)pos[j] & 63u));
+            if (pos[j] >= 0)               /* (what is no page of the pool would wrap to one from 2^26 on) */
+                slot[j] = (unsigned)slot[j] < (unsigned)A.n_pages ? (int)(((unsigned)slot[j] << kPlanPageShift) + ((unsigned)pos[j] & 63u)) : -1;
 #pragma unroll
         for (int j = 0; j < kRun; j += 4) {
             if (vec && r0 + j + 4 <= max_rows) {
