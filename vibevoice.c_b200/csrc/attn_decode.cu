@@ -144,13 +144,22 @@ template <int FMT, int HD, int NT> struct AttnShape {
     static constexpr int USED = 2 * ROWS + (kv_is_tq(FMT) ? 8 * F::KEYS : 0);                 /* then the words that hold the rows' RMS values */
     static constexpr int OUT = NT * HD * 32;                                                  /* a warp's output, left in the stage it has read last */
     static constexpr int STAGE = USED > OUT ? USED : OUT;
-    static constexpr int CTAS = F::W == 12 ? 1 : HD == 256 || NT == 2 ? 2 : 3;                /* an SM's, by registers and shared memory */
-    static constexpr int STAGES = FMT == KV_TQ4 || F::VEC * F::KG >= 256 ? 2 : 3;
+    static constexpr int LUT = F::LUT * F::LUT_STEP;
+    /* CTAs that an SM has registers for, and those that it has shared memory for too: the work is cut into a part for
+     * each that is resident at once, and one more would be a wave of its own. Three stages of short rows, where as many
+     * CTAs have room for them. (One CTA of 256-wide FP16 heads, two of 16 heads in 1.5 bits and three of 3 bits in two
+     * stages, against one more that waited for room: 48 sequences of 4100 .. 8200 106.7 -> 100.5, 76.3 -> 52.9 and
+     * 106.4 -> 85.2 us; 3 bits in three stages, two CTAs: 93.4.) */
+    static constexpr int OF_SM = 228 << 10, OF_CTA = 1 << 10;                                 /* shared memory; what the system takes of it */
+    static constexpr int STATIC = (F::W * (16 * NT + 1) * 4 + 4 + 127) / 128 * 128;           /* the kernel's own arrays */
+    static constexpr int BY_REGS = F::W == 12 ? 1 : HD == 256 || NT == 2 ? 2 : 3;
+    static constexpr int STAGES = FMT == KV_TQ4 || F::VEC * F::KG >= 256 || BY_REGS * (LUT + F::W * 3 * STAGE + STATIC + OF_CTA) > OF_SM ? 2 : 3;
     static constexpr int RING = STAGE * STAGES;                                               /* a warp's */
     static constexpr int TILES = HD / 16;                                                     /* 16-dim tiles of the output */
     static constexpr int MINE = (NT * TILES + F::W - 1) / F::W;                               /* of them a warp finishes */
-    static constexpr int LUT = F::LUT * F::LUT_STEP;
     static constexpr int SMEM = LUT + F::W * RING;                                            /* in this order */
+    static constexpr int BY_SMEM = OF_SM / (SMEM + STATIC + OF_CTA), CTAS = BY_REGS < BY_SMEM ? BY_REGS : BY_SMEM;
+    static_assert(CTAS > 0, "a CTA fits an SM");
 };
 
 /* ---------------------------------------------------------------- instructions */
