@@ -1101,7 +1101,9 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
     const int per = A.by_item ? 1 : kAttnJoinParts, mine = blockIdx.x * per + lane;
     int2 d = make_int2(-1, 0);
     if (lane < per && (A.by_item || mine < A.parts)) d = A.desc[mine];
-    unsigned todo = __ballot_sync(0xffffffffu, d.x >= 0);
+    /* (a scratch that another call has written to in between must not lead outside of it) */
+    const int limit = A.by_item ? A.parts : A.n_seqs * A.n_kv * A.head_blocks;
+    unsigned todo = __ballot_sync(0xffffffffu, (unsigned)d.x < (unsigned)limit && (unsigned)d.y <= (unsigned)(A.by_item ? d.x : mine));
     for (int n = 0; todo != 0; todo &= todo - 1) {
         const int i = __ffs(todo) - 1, which = blockIdx.x * per + i;
         const int dx = __shfl_sync(0xffffffffu, d.x, i), first = __shfl_sync(0xffffffffu, d.y, i);
