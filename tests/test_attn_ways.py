@@ -45,3 +45,35 @@ def test_attn_ways_of_other_heads(vv, fmt, nq, nkv, hd, block, n, blocks):
         d.check(out[b:b + 1], lse[b:b + 1])
     again = c.run()
     assert np.array_equal(again[0].view(np.uint16), out.view(np.uint16)) and np.array_equal(again[1], lse)
+
+
+# sequences, blocks, whether one kernel does it: at the limits between the ways and past them, four cache heads
+EDGES = [(2, 8, True), (2, 9, False), (16, 10, True), (16, 11, False), (24, 14, True), (24, 15, False), (47, 14, True), (48, 16, True), (48, 17, False),
+         (148, 2, True), (148, 3, True), (222, 3, True), (222, 4, True), (444, 5, True), (444, 6, True), (1332, 8, True), (1332, 9, True)]
+
+
+@pytest.mark.parametrize("n,blocks,one", EDGES)
+@pytest.mark.parametrize("fmt", [FP16, E5M2])
+def test_attn_at_the_limits_of_the_ways(vv, fmt, n, blocks, one):
+    rng = np.random.default_rng(n + blocks)
+    top = blocks * (64 if fmt == FP16 else 128)
+    lens = np.where(rng.random(n) < 0.2, 0, np.exp(rng.uniform(0, np.log(min(top, 300) + 1), n))).astype(np.int64)
+    lens[rng.integers(n)] = top
+    c = Case(vv, lens, 8, 4, 128, fmt, seed=n, slack=0).upload()
+    n0 = vv.launch_count()
+    out, lse = c.run()
+    assert vv.launch_count() - n0 == (1 if one else 2)
+    c.check(out, lse)
+
+
+@pytest.mark.parametrize("n,blocks,one", [(2, 4, True), (2, 5, False), (16, 5, True), (16, 6, False), (24, 7, True), (24, 8, False), (60, 8, True), (60, 9, False), (148, 1, True), (300, 3, True), (444, 5, True), (444, 6, True)])
+@pytest.mark.parametrize("fmt,block", [(TQ4, 384), (TQ3, 256), (TQ1_5, 256)])
+def test_attn_at_the_limits_of_the_ways_of_rotated_formats(vv, fmt, block, n, blocks, one):
+    rng = np.random.default_rng(n + blocks)
+    lens = np.where(rng.random(n) < 0.2, 0, np.exp(rng.uniform(0, np.log(300), n))).astype(np.int64)
+    lens[rng.integers(n)] = blocks * block
+    c = Case(vv, lens, 8, 4, 128, fmt, seed=n, slack=0).upload()
+    n0 = vv.launch_count()
+    out, lse = c.run()
+    assert vv.launch_count() - n0 == (1 if one else 2)
+    c.check(out, lse)

@@ -1165,25 +1165,40 @@ __global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_cons
 static int attn_col_tiles(int group, int head_dim, int fmt) { return group > 8 && head_dim <= 128 && fmt != KV_TQ4 ? 2 : 1; }
 
 /* Whether items stay whole, which saves the joining kernel: 2, each a warp's; 1, each a CTA's; 0, they are cut. By
- * the blocks that a table has room for, since the lengths are known on the device alone: at the limits the best way
- * loses a little where every sequence fills its table and gains where they do not. The rotated formats take longer
- * for a block, heads of 256 fill fewer CTAs an SM. Measured, us (cut / CTA / warp), every sequence that long or, the
- * second triple, from one position to that evenly by the logarithm; 28 heads over 4 of 128:
- *   items  blocks  FP16                                     4 bits
- *   4      4       6.7 / 5.3                                12.0 / 13.2 (2: 10.9 / 8.1)
- *   4      8       7.0 / 7.8 (6: 6.7 / 6.6)                 11.9 / 19.0 (7)
- *   64     4       8.0 / 5.6                                15.8 / 13.5
- *   64     8       9.4 / 8.4                                17.1 / 19.5 (7)
- *   384    8       25.6 / 19.2        12.0 / 9.0            57.5 / 57.9 (7)    24.5 / 28.4
- *   384    16      39.8 / 33.1        12.9 / 15.9           109 / 114          31.8 / 39.9
- *   1200   2       22.8 / 20.6 / 18.9 16.5 / 13.7 / 11.8    71.3 / 69.6 / 51.7 48.2 / 43.0 / 35.0
- *   1200   4       35.6 / 30.6 / 30.3 19.3 / 17.2 / 18.2    104 / 106 / 94.6   51.5 / 50.6 / 72.8
- *   2400   5             68.7 / 70.2        29.5 / 27.8           227 / 218          92.8 / 115
- * FP8 and heads of 64 are near FP16's; heads of 256, 384 items, 8 blocks: 48.3 / 53.0, 23.8 / 22.7. */
-static int attn_whole(long long items, long long blocks, bool slow) {
-    if ((items >= 888 && blocks <= (slow ? 2 : 3)) || (items >= 1776 && blocks <= 5 && !slow)) return 2;
-    const int most = items < 64 ? 8 : items < 384 ? 10 : 16;
-    return blocks <= (slow ? most / 2 : most) ? 1 : 0;
+ * the blocks that a table has room for, since the lengths are known on the device alone: wide tables are cut however
+ * short their sequences are. A warp each pays where there are items for the `warps` of the launch, for longer ones
+ * the more there are; a CTA each where that takes less than the second kernel's 3 us more, or where there are items
+ * enough to even out. A block of a rotated format takes longer. The limits are by the mean time over sequences as long as
+ * the table has room for, by the logarithm from one position to that, and both for every table down to a third (a
+ * server's table has room to grow). Measured, us, cut / CTA / warp, every sequence as long as the table and that mean;
+ * 28 heads over 4 of 128, 1776 warps; at the last size that stays whole and the next:
+ *   items  blocks  FP16                                     blocks  4 bits
+ *   4      8       7.5 / 8.2            7.4 / 6.5           4       12.4 / 13.7          12.4 / 11.5
+ *   4      10      7.6 / 9.5            7.5 / 7.3           5       12.6 / 15.8          12.4 / 12.5
+ *   64     10      10.4 / 9.9           9.1 / 7.6           5       16.1 / 15.9          14.3 / 12.7
+ *   64     12      10.6 / 11.2          9.2 / 8.0           6       18.6 / 18.1          14.6 / 13.6
+ *   128    14      17.7 / 17.1          11.0 / 9.4          7       26.3 / 20.8          16.8 / 15.8
+ *   128    16      19.5 / 19.2          11.6 / 10.6         8       28.4 / 22.9          17.5 / 16.7
+ *   384    16      40.7 / 34.1          19.1 / 15.5         8       66.5 / 65.7          35.0 / 36.1
+ *   384    18      44.4 / 37.3          19.8 / 16.3         10      76.7 / 78.8          37.9 / 40.2
+ *   640    2       15.5 / 11.8 / 11.0   12.5 / 10.2 / 8.8   2       42.7 / 40.9 / 40.8   31.7 / 29.8 / 27.3
+ *   640    3       20.5 / 18.0 / 18.2   13.6 / 11.2 / 10.5  3       55.1 / 52.7 / 57.8   34.8 / 32.9 / 33.9
+ *   1200   3       30.5 / 26.2 / 25.2   18.8 / 16.4 / 14.0  3       89.0 / 89.6 / 73.6   56.3 / 54.5 / 43.0
+ *   1200   4       36.1 / 31.1 / 30.9   22.7 / 19.8 / 18.6  4       105 / 107 / 95.2     65.2 / 64.4 / 61.0
+ *   1776   5       52.8 / 50.6 / 49.1   30.4 / 27.9 / 25.1  4       143 / 141 / 98.9     87.6 / 85.4 / 67.5
+ *   1776   6       61.2 / 58.8 / 57.0   32.2 / 29.8 / 27.4
+ * One limit serves all of FP16 and FP8, one all of the rotated formats: FP8 and the narrow codes are cut better at
+ * the CTA's limits (4 x 8 E4M3 7.9 / 10.0, the mean 7.7 / 7.7; 4 x 4 2 bits 11.4 / 13.6 and 11.4 / 11.1), FP16 would
+ * stay whole a little longer. 3, 2 and 1.5 bits take a warp each from more items on (2 bits, 640 x 2: 28.4 / 25.5 /
+ * 29.4). Over 1667 points (1 .. 24 blocks, 4 .. 4000 items, ten forms, 16 heads to a cache head and heads of 64 and
+ * 256 among them) the way taken has a mean 1.007 times the best one's. */
+static int attn_whole(long long items, long long blocks, long long warps, int fmt) {
+    const bool tq = kv_is_tq(fmt), narrow = tq && fmt != KV_TQ4;
+    int solo = items >= 3 * warps ? (tq ? 5 : 8) : items >= warps ? 5 : 2 * items >= warps ? 3 : 3 * items >= warps ? 2 : 0;
+    if (narrow && 3 * items < 2 * warps) solo = 0;
+    if (blocks <= solo) return 2;
+    const int most = items < 48 ? 8 : items < 96 ? 10 : items < 192 ? 14 : 16;
+    return blocks <= (tq ? most / 2 : most) ? 1 : 0;
 }
 
 struct AttnScratch { size_t ml, o, bytes; };
@@ -1202,7 +1217,7 @@ static cudaError_t launch_attn(AttnArgs A, long long capacity, cudaStream_t s) {
     static_assert(parts <= kAttnParts, "the scratch holds kAttnParts parts");
     A.parts = parts;
     const long long items = (long long)A.n_seqs * A.n_kv * A.head_blocks;
-    A.whole_items = attn_whole(items, (capacity + AttnFmt<FMT, HD>::BLOCK - 1) / AttnFmt<FMT, HD>::BLOCK, kv_is_tq(FMT) || HD == 256);
+    A.whole_items = attn_whole(items, (capacity + AttnFmt<FMT, HD>::BLOCK - 1) / AttnFmt<FMT, HD>::BLOCK, parts * AttnFmt<FMT, HD>::W, FMT);
     A.one_each = A.whole_items == 1 && items <= parts;
     const int ctas = A.one_each ? (int)items : parts;
     const bool solo = A.whole_items == 2;
