@@ -1092,7 +1092,8 @@ struct AttnState {                                     /* a lane's: maximum and 
     }
 };
 template <int FMT, int HD, int NT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) attn_join_kernel(const __grid_constant__ AttnArgs A) {
+/* (24 warps an SM: the look-up of infinities must not take registers from what hides the loads' latency) */
+__global__ void __launch_bounds__(32 * WARPS, 24 / WARPS) attn_join_kernel(const __grid_constant__ AttnArgs A) {
     constexpr int TILES = HD / 16;
     __shared__ float4 ml_s[WARPS][32], o_s[WARPS][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
