@@ -324,13 +324,16 @@ vv_status_t vvb_kv_rotate_dev(void* x_fp16, int n_heads, int head_dim, int rows,
 vv_status_t vvb_kv_unrotate_dev(void* x_fp16, int n_heads, int head_dim, int rows, void* stream);
 
 /* ---- serving: many sequences over one paged cache ------------------------ *
- * One decode or mixed step over the pool of 64-position pages: vvb_kv_plan_dev
- * gives each sequence the pages its new tokens need and says where every row of
- * the ragged batch goes; per layer, vvb_kv_append_slots_dev rotates and stores
- * those rows and vvb_attn_decode_dev attends each sequence's newest token to its
- * whole cache. Rows of a ragged batch lie one sequence after the other. All
- * three are capturable: lengths, tables and maps are read on the device, so a
- * replayed graph follows them. */
+ * One step over the pool of 64-position pages: vvb_kv_plan_dev gives each sequence
+ * the pages its new tokens need and says where every row of the ragged batch goes;
+ * per layer, vvb_kv_append_slots_dev rotates and stores those rows and
+ * vvb_attn_decode_dev attends each sequence's newest token to its whole cache.
+ * That is all of a step of one new token per sequence. Of a sequence with several (a
+ * prompt or a chunk of one) it is the cache and the newest token alone: the
+ * attention of its other rows, which the next layer needs, is not among these
+ * calls. Rows of a ragged batch lie one sequence after the other. All three are
+ * capturable: lengths, tables and maps are read on the device, so a replayed graph
+ * follows them. */
 
 /** What vvb_kv_plan_dev says of a sequence (status[b]). A refused sequence keeps
  *  its length and pages; its rows get slot -1. */
@@ -385,7 +388,9 @@ vv_status_t vvb_kv_plan_dev(const vvb_kv_plan_t* plan, void* stream);
  *  left alone: no cache row, no q_out row is written. Two rows must not name the
  *  same slot. k_ref is one reference key for all sequences (the attention's
  *  softmax does not change with it; its log-sum-exp is then of the stored
- *  differences). Alignment and head_dim as vvb_kv_append_dev. */
+ *  differences). Rows without a slot are read all the same: a batch that is mostly
+ *  padding takes the time of a full one, but for the stores. Alignment and head_dim
+ *  as vvb_kv_append_dev. */
 typedef struct vvb_kv_append_slots {
     const void* q;             /* [rows, n_q_heads, head_dim] */
     void* q_out;               /* [rows, n_q_heads, head_dim]; q is allowed */
@@ -413,22 +418,26 @@ vv_status_t vvb_kv_append_slots_dev(const vvb_kv_append_slots_t* args, void* str
  *  token's among them), query head h reading cache head h / (n_q_heads / n_kv_heads),
  *    s_j = scale * q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),
  *    lse = m + ln sum_j e^(s_j - m),  m = max_j s_j,
- *  every sum, the maximum and the scores in FP32. A sequence without keys (or a
+ *  every sum, the maximum and the scores in FP32, a weight as two FP16 values (22
+ *  bits, nothing below 2^-37 of the largest), the levels of a rotated format as FP16
+ *  values within 9e-5 of themselves (1.5 bits: 1.6e-4). A sequence without keys (or a
  *  head all of whose scores are -inf) gets zeros and lse = -inf. An infinity in V has
  *  its sign in the result, however small its weight is beside the others'.
  *  Key j lies in cache row block_table[b][j / 64] * 64 + j % 64, or with
  *  block_table == NULL in row b * table_stride + j (table_stride: rows of the
  *  cache per sequence). n is cut to the 64 * table_stride (table_stride) positions
  *  that there are, and to 0 below it; keys whose row lies outside [0, n_slots)
- *  are left out as if masked. Whatever the rows beyond n hold, NaN included, has no effect. A
- *  single sequence of the contiguous cache takes lens = its device position
+ *  are left out as if masked. Whatever the rows beyond n hold, NaN included, has no
+ *  effect. A single sequence of the contiguous cache takes lens = its device position
  *  (vvb_kv_append_dev's d_position) and len_add = 1.
- *  TurboQuant caches hold rotated vectors: q is what vvb_kv_rotate_dev made of it and out is
- *  what vvb_kv_unrotate_dev takes, as in the reference (src/inference/decoder.c:878-901).
+ *  TurboQuant caches hold rotated vectors: q is what vvb_kv_rotate_dev made of it and
+ *  out is what vvb_kv_unrotate_dev takes, as in the reference
+ *  (src/inference/decoder.c:878-901).
  *  A reference key (k_ref) shifts all scores of a head alike and is not needed.
  *  head_dim 64, 128 or 256 (TurboQuant: 128); n_q_heads a multiple of n_kv_heads;
  *  q, out, the stores and scratch 16-byte aligned, k_meta and v_meta 4-byte
- *  aligned (VV_ERR_UNSUPPORTED otherwise); n_seqs <= 8192, n_q_heads <= 4096. out may be q. scratch:
+ *  aligned (VV_ERR_UNSUPPORTED otherwise); n_seqs <= 8192, n_q_heads <= 4096. out may
+ *  be q. scratch:
  *  vvb_attn_decode_scratch_bytes(...) bytes of device memory whose contents need
  *  no initialisation; calls that overlap on a GPU need one each (two captured
  *  graphs may share one when they do not run at the same time). The work is

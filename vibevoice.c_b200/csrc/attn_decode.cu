@@ -29,30 +29,35 @@
  * FP8: e4m3 by cvt, two to an instruction; e5m2 is the upper half of an FP16
  * value and needs one byte permute. TurboQuant: two codes index a table in
  * shared memory of two FP16 levels, a copy for each lane, so that 32 lanes never
- * meet in a bank. 16 keys of the 4-bit format are 406 instructions a warp, 70 of
- * them such look-ups (FP16: 296, no look-ups): it is issue-bound, its ALU pipe first
- * (tried: entries 128 bytes apart, three CTAs of four warps with a table each:
- * 61.6 us for 48 sequences of 4100 - 8200; 256 apart, where one byte permute
- * forms the address, and twelve warps over one table: 58.9; fourteen and sixteen
- * warps of fewer registers: 69, 84).
+ * meet in a bank. 16 keys of the 4-bit format are 417 instructions a warp, all told,
+ * 71 of them reads of shared memory (smsp__inst_executed over the groups of 48
+ * sequences; FP16 328, E4M3 272): it is bound by its instructions and the latencies
+ * between them, issue slots 52 % busy, three warps a scheduler (tried: entries 128
+ * bytes apart, three CTAs of four warps with a table each: 61.6 us for 48 sequences
+ * of 4100 - 8200; 256 apart, where one byte permute forms the address, and twelve
+ * warps over one table: 58.9; fourteen and sixteen warps of fewer registers: 69, 84).
  *
  * Work: the blocks of 64 (128, 256, 384) positions of all items in one line, cut
  * into equal parts, one for each CTA that fits the GPU at once. The cut depends
  * on the lengths alone, which every warp sums up on the device, so the same
  * inputs give the same bits. (A line of less than 2^22 places is cut in 32-bit
  * numbers without a long division ahead of the first load: 0.45 us a call.) The
- * CTA's warps share each block. An item that a CTA holds whole is finished by it, the warps' outputs exchanged in the ring's
- * stage read last; of one that is cut, each CTA leaves its part (running maximum,
- * sum, output) in scratch and a second kernel joins them. attn_whole says when
- * items stay whole instead and the second kernel is saved.
+ * CTA's warps share each block. An item that a CTA holds whole is finished by it,
+ * the warps' outputs exchanged in the ring's stage read last; of one that is cut,
+ * each CTA leaves its part (running maximum, sum, output) in scratch and a second
+ * kernel joins them. attn_whole says when items stay whole instead and the second
+ * kernel is saved: by the room in the block tables, not by the lengths.
  *
- * Measured (28 heads over 4, 128 wide; GB/s of K and V): 64 x 4096 FP16 85.8 us
- * = 6.26 TB/s, 0.95 of the device's copy rate; 96 sequences of 1 .. 16384 57.6 us,
- * 0.85; 48 of 4100 .. 8200 in FP8 53.5 us, 0.85; the same in 4 bits 58.9 us, 0.40;
- * 1 x 14449 FP16 11.9 us, latency: the first loads behind lens and table, three
- * steps, and the join; 1 x 300 6.0, 1 x 64 3.5, whole items in one kernel. Bytes in
- * flight: one stage of 8 KB for each of 12 warps an SM beside the one being read; two stages are slower (89.4 us for 64 x 4096),
- * and so are two CTAs an SM (88.3).
+ * Measured, replayed from a graph (28 heads over 4, 128 wide; GB/s of K and V):
+ * 64 x 4096 FP16 87.9 us (86.2 .. 88.7 by box) = 6.11 TB/s, 0.93 of the device's
+ * copy rate; 96 sequences of 1 .. 16384 58.1 us, 0.83; 48 of 4100 .. 8200 in E4M3
+ * 55.0 us, 0.83; the same in 4 bits 60.6 us, 0.39, in 3 bits 83.7, 2 bits 62.6, 1.5
+ * bits 71.8; 1 x 14449 FP16 12.4 us, latency: the first loads behind lens and
+ * table, three steps, and the join. With tables of little more room than the
+ * sequence, whole items in one kernel: 1 x 300 6.1, 1 x 64 3.6; with tables of 512
+ * pages, cut: 7.2, 5.9. Bytes in flight: one stage of 8 KB for each of 12 warps an
+ * SM beside the one being read; two stages are slower (64 x 4096 89.4 us where one
+ * was 86.0), and so are two CTAs an SM (88.3).
  * A cluster of eight CTAs for an item, joined through distributed shared memory
  * in one launch, costs more than the second kernel (1 x 300, cut: 8.4 us, 7.1).
  *
@@ -62,13 +67,14 @@
  * output's own rounding; below 2^-37 of the largest a weight is nothing. An infinity
  * in V meets two positive factors where its weight is 2^-20 of the largest or more
  * (weight_rest); under less it can make the sum a NaN, which is then looked up
- * (attn_infinite). The
- * maximum follows the scores only beyond a factor of 2^3 (8 % of the steps instead of 41 % for normal scores over 600 keys): 2^15 is the largest
- * weight then. For the rotated
- * formats the levels times a common factor become FP16 values within 9e-5 of
- * themselves (attn_alpha, found by trying factors in [1, 2); 1.6e-4 for the
- * 1.5-bit code words), the RMS of a key multiplies its score, the RMS of V the
- * weight, relative to a power of two that follows the largest RMS.
+ * (attn_infinite). The maximum follows the scores only beyond a factor of 2^3 (8 %
+ * of the steps instead of 41 % for normal scores over 600 keys): 2^15 is the
+ * largest weight then. For the rotated formats the levels times a common factor
+ * become FP16 values within 9e-5 of themselves (attn_alpha, found by trying factors
+ * in [1, 2); 1.6e-4 for the 1.5-bit code words), since the product takes FP16: it
+ * costs 2.8e-4 of the output where its own rounding is 2.1e-4. The RMS of a key
+ * multiplies its score, the RMS of V the weight, relative to a power of two that
+ * follows the largest RMS.
  */
 #include "fp8_kv.cuh"
 #include "tq_kv.cuh"
