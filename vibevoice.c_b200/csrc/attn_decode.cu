@@ -507,15 +507,22 @@ template <int FMT> __device__ __forceinline__ bool attn_code_negative(const uint
     const unsigned c = (w >> (bit & 7)) & ((1u << NB) - 1u);
     return FMT == KV_TQ1_5 ? c_vq15[2 * c + (dim & 1)] < 0.0f : c < (1u << (NB - 1));
 }
-/* What a NaN in an output stands for whose scores are no NaN: infinities in V, which have their sign in the result
- * under any weight of a finite score, but are NaN where the weight, or a half of it, is 0 in FP16 or in FP32. So V
- * is looked through at that dim, a key at a time: it happens to infinite values only. (Infinities of both signs and
- * NaNs give NaN. V of a key whose score is -inf counts as any.) */
-template <int FMT, int HD> __device__ float attn_infinite(const AttnArgs& A, int b, int hk, int dim) {
+/* Outputs that attn_out has marked, of `heads` heads of cache head hk of sequence b, at sixteen dims; by a warp, once
+ * they are all written. What such a NaN stands for are infinities in V: they have their sign in the result under any
+ * weight of a finite score, but are NaN where the weight, or a half of it, is 0 in FP16 or in FP32. So V is looked
+ * through at those dims, a key a lane. That happens to infinite values only, and takes what reading V of sixteen
+ * dims by one warp does: 64 x 4096 255 us with infinities in one dim, 637 in all, 1 x 14449 320. (Infinities of both signs and NaNs give NaN. V of a key whose score is -inf counts as any.) */
+template <int FMT, int HD, typename Dim>
+__device__ __forceinline__ void attn_infinite(const AttnArgs& A, int b, int hk, __half* out, int heads, Dim dim_of, int lane) {
     constexpr int VEC = AttnFmt<FMT, HD>::VEC;
+    const int mine = dim_of(lane & 15);
+    bool marked = false;
+    for (int h = lane >> 4; h < heads; h += 2) marked |= __half_as_ushort(out[h * HD + mine]) == kAttnMark;
+    if (!__any_sync(0xffffffffu, marked)) return;
     const int n = attn_keys(A, b);
-    bool pos = false, neg = false, nan = false;
-    for (int j = 0; j < n && !nan && !(pos && neg); j++) {
+    unsigned pos = 0, neg = 0, nan = 0;                /* a bit a dim */
+#pragma unroll 1
+    for (int j = lane; j < n; j += 32) {
         long long row = (long long)b * A.table_stride + j;
         if (A.block_table != nullptr) {
             const int page = __ldg(A.block_table + (size_t)b * A.table_stride + (j >> kAttnPageShift));
@@ -526,28 +533,37 @@ template <int FMT, int HD> __device__ float attn_infinite(const AttnArgs& A, int
         const size_t at = (size_t)row * A.n_kv + hk;
         if constexpr (kv_is_tq(FMT)) {
             const float rms = __half2float(A.v_meta[at]);
-            nan |= rms != rms;
-            if (rms == INFINITY) (attn_code_negative<FMT>(A.v_store + at * VEC, dim) ? neg : pos) = true;
+            if (rms != rms) nan = 0xffffu;
+            if (rms == INFINITY)
+                for (int k = 0; k < 16; k++) (attn_code_negative<FMT>(A.v_store + at * VEC, dim_of(k)) ? neg : pos) |= 1u << k;
         } else {
-            const float v = FMT == KV_RAW ? __half2float(reinterpret_cast<const __half*>(A.v_store)[at * HD + dim])
-                                          : __half2float(__ushort_as_half((unsigned short)(A.v_store[at * VEC + dim] << 8)));
-            nan |= v != v;
-            pos |= v == INFINITY;
-            neg |= v == -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const float v = FMT == KV_RAW ? __half2float(reinterpret_cast<const __half*>(A.v_store)[at * HD + dim_of(k)])
+                                              : __half2float(__ushort_as_half((unsigned short)(A.v_store[at * VEC + dim_of(k)] << 8)));
+                nan |= (v != v ? 1u : 0u) << k;
+                pos |= (v == INFINITY ? 1u : 0u) << k;
+                neg |= (v == -INFINITY ? 1u : 0u) << k;
+            }
         }
     }
-    return nan || pos == neg ? __int_as_float(0x7fffffff) : pos ? INFINITY : -INFINITY;
+    pos = __reduce_or_sync(0xffffffffu, pos);
+    neg = __reduce_or_sync(0xffffffffu, neg);
+    nan = __reduce_or_sync(0xffffffffu, nan) | ~(pos ^ neg);
+    const unsigned bit = 1u << (lane & 15);
+    if (nan & bit) return;
+    for (int h = lane >> 4; h < heads; h += 2)
+        if (__half_as_ushort(out[h * HD + mine]) == kAttnMark) out[h * HD + mine] = __ushort_as_half(pos & bit ? 0x7c00 : 0xfc00);
 }
-/* Outputs of items first .. last (whole ones, by their places in the line) that attn_out has marked. Called once they
- * are all written, by `threads` threads, so that what it takes is not paid for where there are none. */
-template <int FMT, int HD> __device__ __noinline__ void attn_look_up(const AttnArgs& A, int first, int last, int heads_of, int thread, int threads) {
+/* All outputs of items first .. last (whole ones, by their places in the line), by warps `warp` of `warps`. */
+template <int FMT, int HD> __device__ __noinline__ void attn_look_up(const AttnArgs& A, int first, int last, int heads_of, int warp, int warps) {
     const int items = A.n_kv * A.head_blocks;
     for (int i = first; i <= last; i++) {
         const int b = i / items, h = i - b * items, hk = h / A.head_blocks, h0 = (h - hk * A.head_blocks) * heads_of;
         if (attn_keys(A, b) == 0) continue;            /* zeros, perhaps another CTA's, and perhaps not written yet */
-        __half* const o = A.out + ((size_t)b * A.n_q + (size_t)hk * A.group + h0) * HD;
-        for (int e = thread; e < min(heads_of, A.group - h0) * HD; e += threads)
-            if (__half_as_ushort(o[e]) == kAttnMark) o[e] = __float2half(attn_infinite<FMT, HD>(A, b, hk, e % HD));
+        __half* const out = A.out + ((size_t)b * A.n_q + (size_t)hk * A.group + h0) * HD;
+        for (int d0 = 16 * warp; d0 < HD; d0 += 16 * warps)
+            attn_infinite<FMT, HD>(A, b, hk, out, min(heads_of, A.group - h0), [d0](int k) { return d0 + k; }, threadIdx.x & 31);
     }
 }
 
@@ -1072,7 +1088,7 @@ __global__ void __launch_bounds__(32 * AttnFmt<FMT, HD>::W, AttnShape<FMT, HD, N
         if (SOLO ? __any_sync(0xffffffffu, odd) : __syncthreads_or(odd)) {
             const int last = at.b * items + at.h - (SOLO || at.last() ? 0 : 1);
             if (SOLO) __syncwarp();                    /* (all outputs are written; a barrier does it for the CTA) */
-            attn_look_up<FMT, HD>(A, first_s[SOLO ? warp : 0], last, 8 * NT, SOLO ? lane : tid, SOLO ? 32 : 32 * W);
+            attn_look_up<FMT, HD>(A, first_s[SOLO ? warp : 0], last, 8 * NT, SOLO ? 0 : warp, SOLO ? 1 : W);
         }
     }
 }
@@ -1146,23 +1162,19 @@ __global__ void __launch_bounds__(32 * WARPS, 24 / WARPS) attn_join_kernel(const
         const int b = item / items, it = item - b * items, hk = it / A.head_blocks, hb = it - hk * A.head_blocks;
         const int heads = A.group - hb * 8 * NT;
         const size_t head0 = (size_t)b * A.n_q + (size_t)hk * A.group + hb * 8 * NT;
+        bool odd = false;
 #pragma unroll
         for (int c = 0; c < 2; c++) {
             const int h = 8 * nt + 2 * t + c;
             if (h >= heads) continue;
-            bool odd = false;
-            const uint32_t two = attn_out(s.o[c], s.o[c + 2], s.l[c], odd);
-            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, two);
+            attn_store<FMT>(A.out + (head0 + h) * HD, j, g, attn_out(s.o[c], s.o[c + 2], s.l[c], odd));
             if (A.lse != nullptr && j == 0 && g == 0) A.lse[head0 + h] = attn_lse(s.m[c], s.l[c]);
-            if constexpr (FMT != KV_E4M3) {
-                if (!odd) continue;
-#pragma unroll 1
-                for (int e = 2 * j; e < 2 * j + 2; e++) {
-                    const int dim = attn_v_dim<FMT>(e, g);
-                    __half* const out = A.out + (head0 + h) * HD + dim;
-                    if (__half_as_ushort(*out) == kAttnMark) *out = __float2half(attn_infinite<FMT, HD>(A, b, hk, dim));
-                }
-            }
+        }
+        if constexpr (FMT != KV_E4M3) {
+            if (!__any_sync(0xffffffffu, odd)) continue;
+            __syncwarp();                              /* the tile's outputs are all written by this warp */
+            attn_infinite<FMT, HD>(A, b, hk, A.out + (head0 + 8 * nt) * HD, min(8, heads - 8 * nt),
+                                   [j](int k) { return attn_v_dim<FMT>(2 * j + (k & 1), k >> 1); }, lane);
         }
     }
 }
