@@ -457,7 +457,7 @@ typedef struct vvb_attn_decode {
     size_t scratch_bytes;
     int n_seqs, n_q_heads, n_kv_heads, head_dim, n_slots, table_stride, len_add;
     int kv_format;
-    float scale;               /* usually 1 / sqrt(head_dim) */
+    float scale;               /* usually 1 / sqrt(head_dim); finite, and so when taken to base 2 */
 } vvb_attn_decode_t;
 
 size_t vvb_attn_decode_scratch_bytes(int n_seqs, int n_q_heads, int n_kv_heads, int head_dim);

@@ -167,7 +167,7 @@ vv_status_t vvb_attn_decode_dev(const vvb_attn_decode_t* a, void* stream) {
     if (!a) return VV_ERR_NULL_PTR;
     if (!a->q || !a->out || !a->k_store || !a->v_store || !a->lens || !a->scratch) return VV_ERR_NULL_PTR;
     if (a->n_seqs < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->head_dim <= 0 || a->n_slots < 0 ||
-        a->table_stride < 1 || a->n_q_heads % a->n_kv_heads != 0 || !isfinite(a->scale))
+        a->table_stride < 1 || a->n_q_heads % a->n_kv_heads != 0 || !isfinite(a->scale * 1.4426950f))     /* (to base 2) */
         return VV_ERR_INVALID_ARG;
     if (a->kv_format < VVB_KV_FP16 || a->kv_format > VVB_KV_TQ1_5) return VV_ERR_UNSUPPORTED;
     const int tq = a->kv_format >= VVB_KV_TQ4;
